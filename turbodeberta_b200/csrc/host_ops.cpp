@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <unordered_map>
@@ -1337,6 +1338,8 @@ Tables* call_tables(const OptTensor& kr, const OptTensor& qr, const Tensor& q, c
                     (int)((2 * exp_delta_max + 1 + 7) / 8 * 8), true};
 }
 
+#include "host_train.h"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1382,4 +1385,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mask_rows", &mask_rows);
   m.def("pack_rows", &pack_rows);
   m.def("unpack_rows", &unpack_rows);
+  m.def("dropout", &dropout);
+  m.def("norm", &norm);
 }

@@ -120,6 +120,29 @@ struct ShortStack {
   int32_t *status, *counter, *gave_up;                // as in AttnParams; counter[0] and counter[3] are zero on entry and again at the end
   uint64_t limit_ns;                                  // of a wait, after which the kernel gives up
 };
+
+// How one call drops elements (philox.cuh).
+struct Dropout {
+  const int64_t* seed;                                // device word, or null: seed_value (a word can change between replays of a graph)
+  int64_t seed_value, offset;
+  uint32_t drop;                                      // of 65536 numbers; 0: nothing is dropped
+  float scale;                                        // of what stays; 0 where nothing does
+};
+
+// LayerNorm(x), or with `res` LayerNorm(dropout(x) + res), and its backward pass.  Rows of `cols` contiguous elements of one type, `*_stride`
+// elements apart; what is written is contiguous.  Weights and their gradients: of w_dtype.
+struct Norm {
+  const void *x, *res, *w, *b, *dy;
+  int64_t x_stride, res_stride, dy_stride, rows;
+  int cols, w_dtype;
+  float eps;
+  Dropout drop;
+  float* stats;                                       // [rows, 2]: mean, 1 / deviation; written going forward (may be null), read coming back
+  void* y;
+  void *dx, *dres;                                    // without dropout the gradients of x and res are the same: dres alone is written
+  void *dw, *db;
+  float* partial;                                     // tdb_norm_partial_floats(), or null: dw and db are not wanted
+};
 }  // namespace tdb
 
 // What the host extension calls (the checks and the launch behind the tdb_attn_fwd_* entry points on a filled AttnParams,
@@ -154,4 +177,9 @@ TDB_HOST_API int tdb_mask_rows(const void* mask, int elem_bytes, int B, int L, i
                                int32_t* out, void* stream);
 TDB_HOST_API int tdb_mask_positions(const void* mask, int elem_bytes, const int32_t* cu, int B, int L, int32_t* pos, void* stream);
 TDB_HOST_API int tdb_repack(int pack, const void* src, const int32_t* pos, int64_t rows, int row_bytes, void* dst, void* stream);
+// y = dropout(x), n contiguous elements; the gradient of x is the same of the gradient of y.
+TDB_HOST_API int tdb_dropout(const void* x, void* y, int64_t n, int dtype, const tdb::Dropout* d, void* stream);
+TDB_HOST_API int tdb_norm_forward(const tdb::Norm* n, int dtype, void* stream);
+TDB_HOST_API int64_t tdb_norm_partial_floats(int64_t rows, int cols);
+TDB_HOST_API int tdb_norm_backward(const tdb::Norm* n, int dtype, void* stream);
 }
