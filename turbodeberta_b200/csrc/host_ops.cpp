@@ -1387,4 +1387,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("unpack_rows", &unpack_rows);
   m.def("dropout", &dropout);
   m.def("norm", &norm);
+  m.def("lora_linear", &lora_linear);
 }

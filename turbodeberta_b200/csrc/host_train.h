@@ -186,3 +186,137 @@ Tensor norm(const Tensor& x, const OptTensor& res, const Tensor& w, const Tensor
     return NormNode::apply(x, res, w, b, eps, p, seed, seed_value, offset);
   return run_norm(x, res, w, b, eps, d, false).first;
 }
+
+// ----------------------------------------------------------------------------------------------------- projections with adapters
+struct LoraCall {
+  Rows x, dy;
+  Tensor w, bias, a, b, scaling, ids;
+  tdb::Lora l{};
+  LoraCall(const Tensor& x_, const Tensor& w_, const OptTensor& bias_, const Tensor& a_, const Tensor& b_, const OptTensor& scaling_, double scaling_value, const OptTensor& ids_)
+      : x(x_), w(w_.contiguous()), a(a_.contiguous()), b(b_.contiguous()) {
+    l.x = x.ptr(); l.x_stride = x.stride; l.rows = x.rows; l.cols = (int)x.cols;
+    l.features = (int)w.size(0); l.rank = (int)a.size(1); l.n = (int)a.size(0); l.dtype = dtype_code(x_);
+    l.w = w.data_ptr(); l.a = a.data_ptr(); l.b = b.data_ptr();
+    if (bias_) { bias = bias_->contiguous(); l.bias = bias.data_ptr(); }
+    l.scaling_value = (float)scaling_value;
+    if (scaling_) { scaling = scaling_->contiguous(); l.scaling = scaling.data_ptr<float>(); }
+    l.rows_per_id = 1;
+    if (ids_) {
+      ids = ids_->contiguous();
+      l.ids = ids.data_ptr(); l.id_bytes = (int)ids.element_size();
+      if (ids.numel()) l.rows_per_id = l.rows / ids.numel();
+    }
+  }
+  Tensor floats(at::IntArrayRef sizes) const { return at::empty(sizes, w.options().dtype(at::kFloat)); }
+  // The product alone, in fp32.
+  Tensor product(const Tensor& left, const Tensor& right) const {
+    return l.dtype == TDB_DTYPE_F32 ? at::mm(left, right) : at::mm(left, right, at::kFloat);
+  }
+};
+
+// h: the adapters' inner values in the form that the gradient of b is made from, where `keep` asks for them.
+std::pair<Tensor, Tensor> run_lora(LoraCall& c, at::IntArrayRef shape, bool keep) {
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
+  if (c.l.rows == 0) return {at::empty(shape, c.w.options()), c.floats({1, 0, c.l.rank})};
+  const int shares = tdb_lora_shares(&c.l, 0);
+  Tensor h = c.floats({shares, c.l.rows, c.l.rank});
+  check_rc(tdb_lora_shrink(&c.l, 0, h.data_ptr<float>(), shares, stream));
+  const Tensor base = c.product(c.x.t, c.w.t());
+  Tensor y = c.l.dtype == TDB_DTYPE_F32 ? base : at::empty({c.l.rows, c.l.features}, c.w.options());
+  check_rc(tdb_lora_expand(&c.l, 0, base.data_ptr<float>(), h.data_ptr<float>(), shares, y.data_ptr(), stream));
+  return {y.view(shape), keep ? h : Tensor()};
+}
+
+Tensor lora_gradient(const LoraCall& c, bool of_b, const Tensor& v, cudaStream_t stream) {
+  const Tensor& like = of_b ? c.b : c.a;
+  if (c.l.rows == 0) return at::zeros_like(like);
+  const int shares = tdb_lora_gather_shares(&c.l, of_b);
+  Tensor part = c.floats({shares, c.l.n, c.l.rank, of_b ? c.l.features : c.l.cols}), out = at::empty(like.sizes(), like.options());
+  check_rc(tdb_lora_gather(&c.l, of_b, v.data_ptr<float>(), (int)v.size(0), part.data_ptr<float>(), shares, out.data_ptr(), stream));
+  return out;
+}
+
+class LoraNode : public torch::autograd::Function<LoraNode> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias, const Tensor& a, const Tensor& b,
+                        const OptTensor& scaling, double scaling_value, const OptTensor& ids, std::vector<int64_t> shape) {
+    at::AutoDispatchBelowAutograd below;
+    c10::cuda::CUDAGuard guard(x.device());
+    LoraCall c(x, w, bias, a, b, scaling, scaling_value, ids);
+    auto [y, h] = run_lora(c, shape, b.requires_grad());
+    ctx->save_for_backward({x, w, a, b, scaling ? *scaling : Tensor(), ids ? *ids : Tensor(), h});
+    ctx->saved_data["scaling"] = scaling_value;
+    ctx->saved_data["bias"] = bias.has_value();
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    refuse_second_derivative("lora_linear");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &a = saved[2], &b = saved[3], &scaling = saved[4], &ids = saved[5], &h = saved[6];
+    const int at = ctx->saved_data["bias"].toBool() ? 3 : 2;
+    const bool need_x = ctx->needs_input_grad(0), need_a = ctx->needs_input_grad(at), need_b = ctx->needs_input_grad(at + 1);
+    c10::cuda::CUDAGuard guard(x.device());
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
+    LoraCall c(x, w, std::nullopt, a, b, scaling.defined() ? OptTensor(scaling) : std::nullopt, ctx->saved_data["scaling"].toDouble(),
+               ids.defined() ? OptTensor(ids) : std::nullopt);
+    c.dy = Rows(grads[0]);
+    c.l.dy = c.dy.ptr();
+    c.l.dy_stride = c.dy.stride;
+    Tensor dx, da, db, u;
+    if (c.l.rows && (need_x || need_a)) {
+      const int shares = tdb_lora_shares(&c.l, 1);
+      u = c.floats({shares, c.l.rows, c.l.rank});
+      check_rc(tdb_lora_shrink(&c.l, 1, u.data_ptr<float>(), shares, stream));
+    }
+    if (need_x) {
+      if (c.l.rows == 0) {
+        dx = at::empty(x.sizes(), x.options());
+      } else {
+        const Tensor base = c.product(c.dy.t, c.w);
+        dx = c.l.dtype == TDB_DTYPE_F32 ? base : at::empty({c.l.rows, c.l.cols}, c.w.options());
+        check_rc(tdb_lora_expand(&c.l, 1, base.data_ptr<float>(), u.data_ptr<float>(), (int)u.size(0), dx.data_ptr(), stream));
+        dx = dx.view(x.sizes());
+      }
+    }
+    if (need_a) da = lora_gradient(c, false, u, stream);
+    if (need_b) db = lora_gradient(c, true, h, stream);
+    const Tensor none;
+    return {dx, none, none, da, db, none, none, none, none};
+  }
+};
+
+Tensor lora_linear(const Tensor& x, const Tensor& w, const OptTensor& bias, const Tensor& a, const Tensor& b, const OptTensor& scaling, double scaling_value,
+                   const OptTensor& ids) {
+  dtype_code(x);
+  if (x.dim() < 1 || w.dim() != 2 || x.size(-1) != w.size(1)) throw py::value_error("x [..., in] and weight [out, in] do not fit together");
+  const int64_t K = w.size(1), N = w.size(0);
+  if (K < 1 || N < 1) throw py::value_error("weight must not be empty");
+  if (a.dim() != 3 || b.dim() != 3 || a.size(0) < 1 || a.size(1) < 1 || a.size(2) != K || b.size(0) != a.size(0) || b.size(1) != N || b.size(2) != a.size(1))
+    throw py::value_error("lora_a must be [adapters, rank, in] and lora_b [adapters, out, rank]");
+  if (a.size(1) > 256) throw py::value_error("rank " + std::to_string(a.size(1)) + ": up to 256 is supported");
+  if (a.size(0) > 4095) throw py::value_error(std::to_string(a.size(0)) + " adapters: up to 4095 in one call are supported");
+  int_size(K); int_size(N);
+  if (bias && (bias->dim() != 1 || bias->size(0) != N)) throw py::value_error("bias must be a vector of the weight's rows");
+  for (const Tensor* t : {&w, bias ? &*bias : &w, &a, &b})
+    if (t->scalar_type() != x.scalar_type()) throw py::value_error("x, weight, bias, lora_a and lora_b must share a dtype");
+  if (scaling && (scaling->scalar_type() != at::kFloat || scaling->dim() != 1 || scaling->size(0) != a.size(0)))
+    throw py::value_error("scaling must be a number or a float32 vector with one entry per adapter");
+  if (!ids && a.size(0) != 1) throw py::value_error("adapter_ids may be left out with a single adapter only");
+  if (ids) {
+    if (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong) throw py::value_error("adapter_ids must be int32 or int64");
+    const auto lead = x.sizes().slice(0, x.dim() - 1);
+    const bool rows = ids->sizes() == lead, first = lead.size() > 1 && ids->dim() == 1 && ids->size(0) == lead[0];
+    if (!rows && !first) throw py::value_error("adapter_ids must have the shape of x without its last dimension, or one entry for each entry of x's first");
+  }
+  device_of({&x, &w, bias ? &*bias : nullptr, &a, &b, scaling ? &*scaling : nullptr, ids ? &*ids : nullptr});
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = N;
+  if (at::GradMode::is_enabled()) {
+    if (w.requires_grad() || (bias && bias->requires_grad()) || (scaling && scaling->requires_grad()))
+      throw std::runtime_error("turbodeberta_b200: lora_linear trains the adapters and what is in front of them; weight, bias and scaling are frozen and must not require a gradient");
+    if (x.requires_grad() || a.requires_grad() || b.requires_grad()) return LoraNode::apply(x, w, bias, a, b, scaling, scaling_value, ids, shape);
+  }
+  c10::cuda::CUDAGuard guard(x.device());
+  LoraCall c(x, w, bias, a, b, scaling, scaling_value, ids);
+  return run_lora(c, shape, false).first;
+}

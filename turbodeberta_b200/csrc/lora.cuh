@@ -1,0 +1,25 @@
+// What the kernels for adapters share: whose row it is.
+#pragma once
+#include "tdb_internal.h"
+
+namespace tdb {
+
+struct LoraRows {
+  const void* ids;                                   // int32 or int64, one for every rows_per_id rows; null: all rows are adapter 0's
+  int id_bytes;
+  int64_t rows_per_id, rows;
+  int n;                                             // adapters
+  const float* scaling;                              // one for each adapter; null: scaling_value
+  float scaling_value;
+};
+__device__ __forceinline__ float scaling_of(const LoraRows& r, int adapter) { return r.scaling ? r.scaling[adapter] : r.scaling_value; }
+
+// -1 for a row without one: its id is not an adapter's.
+__device__ __forceinline__ int adapter_of(const LoraRows& r, int64_t row) {
+  if (!r.ids) return 0;
+  const int64_t i = r.rows_per_id == 1 ? row : row / r.rows_per_id;
+  const int64_t id = r.id_bytes == 8 ? static_cast<const int64_t*>(r.ids)[i] : static_cast<const int32_t*>(r.ids)[i];
+  return id >= 0 && id < r.n ? (int)id : -1;
+}
+
+}  // namespace tdb

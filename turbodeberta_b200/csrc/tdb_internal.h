@@ -143,6 +143,19 @@ struct Norm {
   void *dw, *db;
   float* partial;                                     // tdb_norm_partial_floats(), or null: dw and db are not wanted
 };
+
+// A shared projection with the adapters of its rows (lora.cu).  a [n, rank, cols], b [n, features, rank] and w [features, cols] contiguous.
+struct Lora {
+  const void *x, *dy;                                 // [rows, cols], [rows, features]: contiguous elements, rows *_stride apart
+  int64_t x_stride, dy_stride, rows;
+  int cols, features, rank, n, dtype;
+  const void *w, *bias, *a, *b;                       // bias may be null
+  const float* scaling;                               // [n], or null: scaling_value
+  float scaling_value;
+  const void* ids;                                    // see LoraRows
+  int id_bytes;
+  int64_t rows_per_id;
+};
 }  // namespace tdb
 
 // What the host extension calls (the checks and the launch behind the tdb_attn_fwd_* entry points on a filled AttnParams,
@@ -182,4 +195,12 @@ TDB_HOST_API int tdb_dropout(const void* x, void* y, int64_t n, int dtype, const
 TDB_HOST_API int tdb_norm_forward(const tdb::Norm* n, int dtype, void* stream);
 TDB_HOST_API int64_t tdb_norm_partial_floats(int64_t rows, int cols);
 TDB_HOST_API int tdb_norm_backward(const tdb::Norm* n, int dtype, void* stream);
+// Adapters beside a shared product, any type and size.  back: from dy through b and a instead of from x through a and b.  h: [shares, rows, rank], the
+// shares to be added up.  base: the product alone, fp32 [rows, columns of y].
+TDB_HOST_API int tdb_lora_shares(const tdb::Lora* l, int back);
+TDB_HOST_API int tdb_lora_shrink(const tdb::Lora* l, int back, float* h, int shares, void* stream);
+TDB_HOST_API int tdb_lora_expand(const tdb::Lora* l, int back, const float* base, const float* h, int shares, void* y, void* stream);
+// The gradient of a (from v = u and x) or of b (from v = h and dy).  part: [shares, n, rank, columns] floats.
+TDB_HOST_API int tdb_lora_gather_shares(const tdb::Lora* l, int of_b);
+TDB_HOST_API int tdb_lora_gather(const tdb::Lora* l, int of_b, const float* v, int v_shares, float* part, int shares, void* out, void* stream);
 }
