@@ -199,3 +199,34 @@ def test_two_runs_streams_and_a_captured_step(dtype):
     again = run(p)
     for got, k in zip(out, ("y", "dx", "da", "db")):
         assert torch.equal(got, again[k]), k
+
+
+@pytest.mark.parametrize("rows,cols,features,rank,n,spread", [(2600, 64, 4096, 16, 128, 1), (20000, 128, 1024, 8, 3, 400), (9000, 576, 2048, 40, 9, 100),
+                                                              (1500, 2048, 320, 64, 200, 1)])
+def test_many_tiles_and_many_adapters_to_a_tile(rows, cols, features, rank, n, spread):
+    """Blocks that take several tiles in turn, with fewer and more steps than there are stages, and from no adapter to 128 in a tile."""
+    p = problem(rows, cols, features, rank, n, B, "none", seed=rows)
+    rs = np.random.RandomState(rows)
+    ids = np.repeat(rs.randint(-1, n, rows // spread + 1), spread)[:rows]
+    ids[rows // 2:rows // 2 + 300] = -1
+    p["ids"] = torch.from_numpy(ids.astype(np.int32)).cuda()
+    got = run(p)
+    flag = {k: t.double() for k, t in p.items() if t.is_floating_point()}
+    own = torch.from_numpy(ids >= 0).cuda()
+    a, b, s = flag["a"], flag["b"], flag["s"]
+    y, dx = flag["x"] @ flag["w"].T + flag["bias"], flag["dy"] @ flag["w"]
+    da, db = torch.zeros_like(a), torch.zeros_like(b)
+    for i in range(n):
+        at = (p["ids"] == i).nonzero()[:, 0]
+        h, u = s[i] * (flag["x"][at] @ a[i].T), s[i] * (flag["dy"][at] @ b[i])
+        y[at] += h @ b[i].T
+        dx[at] += u @ a[i]
+        da[i], db[i] = u.T @ flag["x"][at], flag["dy"][at].T @ h
+    assert own.any() and not own.all()
+    # Sums of up to 4096 random products: the worst-case bound of the other tests is far above what wrong rows or steps would do to a sum of
+    # squares, so here the whole is held against half a step for every element, doubled for the sums' own error.
+    for k, want in (("y", y), ("dx", dx), ("da", da), ("db", db)):
+        assert (got[k].double() - want).norm() <= 2 * HALF[B] * want.norm(), k
+        assert torch.isfinite(got[k]).all()
+    from turbodeberta_b200.ops.flash_attention import check_pending_status
+    check_pending_status()

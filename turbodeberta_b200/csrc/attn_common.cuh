@@ -50,6 +50,8 @@ __host__ __device__ __forceinline__ int64_t partial_tile(const AttnParams& p, in
 int token_map(CUtensorMap* m, const void* ptr, int64_t tokens, int H, int B, int64_t sb, int64_t st, int64_t sh, const char* what);
 // [heads] x [rows] x 64 bf16, boxes of box_rows rows of one head; 128-byte swizzle.
 int table_map(CUtensorMap* m, const void* ptr, int rows, int H, int box_rows, const char* what);
+// [rows] x [cols] bf16, rows `stride` elements apart, boxes of box_rows rows and 64 columns; 128-byte swizzle.
+int bf16_map_2d(CUtensorMap* m, const void* ptr, uint64_t cols, uint64_t rows, uint64_t stride, uint32_t box_rows, const char* what);
 int launch_attn_far(const AttnParams& p, int64_t tiles, int sms, cudaStream_t s);
 
 }  // namespace tdb

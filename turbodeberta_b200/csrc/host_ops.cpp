@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <map>
 #include <mutex>
@@ -264,6 +265,7 @@ py::object Status::report(c10::cuda::CUDAStream stream) {
 }
 
 // Words of every launch with a deferred check, all devices, and of the caller's own report: None, or the largest of each word.
+int standing_slot(int dev);                          // host_train.h; -1: none yet
 py::object drain_pending(Report* own) {
   Words all;
   for (int dev = 0; dev < MAX_DEV; ++dev) {
@@ -274,7 +276,8 @@ py::object drain_pending(Report* own) {
       take.swap(p.pending);
     }
     const bool with_own = own && own->device() == dev;
-    if (take.empty() && !with_own) continue;
+    const int standing = standing_slot(dev);
+    if (take.empty() && !with_own && standing < 0) continue;
     c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
     cudaError_t e = cudaSuccess;
     {
@@ -289,6 +292,7 @@ py::object drain_pending(Report* own) {
     }
     for (const auto& t : take) all.merge(collect(dev, t.slot, t.keep));
     if (with_own) all.merge(own->take());
+    if (standing >= 0) all.merge(collect(dev, standing, true));       // replays of graphs report there without being listed
     cuda_ok(e, "synchronisation");
   }
   return all.to_python();

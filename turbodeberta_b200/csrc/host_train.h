@@ -188,16 +188,66 @@ Tensor norm(const Tensor& x, const OptTensor& res, const Tensor& w, const Tensor
 }
 
 // ----------------------------------------------------------------------------------------------------- projections with adapters
+// Where the product kernels of a device report, calls and recorded graphs alike: words that no call owns, since nothing but a wait that gave up is
+// ever written there.  Each stream that used them since the last check is listed once.
+std::atomic<int> g_standing[MAX_DEV];                // slot + 1
+int standing_slot(int dev) { return g_standing[dev].load() - 1; }
+
+class StandingReport {
+ public:
+  StandingReport(int dev, c10::cuda::CUDAStream stream) : dev_(dev), stream_(stream) {
+    captured_ = at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None;
+    slot_ = standing_slot(dev);
+    if (slot_ < 0 && !captured_) {
+      static std::mutex mu;
+      std::lock_guard<std::mutex> lock(mu);
+      if (g_standing[dev] == 0) g_standing[dev] = acquire(dev) + 1;
+      slot_ = standing_slot(dev);
+    }
+    if (slot_ >= 0) {
+      words = g_pools[dev].host + slot_ * SLOT_WORDS;
+    } else {                                         // the first call of a process is being captured, or every slot is taken
+      own_ = at::zeros({SLOT_WORDS}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)dev));
+      words = own_.data_ptr<int32_t>();
+    }
+  }
+  // Behind the launch.
+  void list() {
+    if (own_.defined()) {
+      py::gil_scoped_acquire gil;
+      py::module_::import("turbodeberta_b200.status").attr("PENDING").attr("append")(own_);
+      return;
+    }
+    if (captured_) return;                           // a check looks at the words in any case
+    StatusPool& p = g_pools[dev_];
+    std::lock_guard<std::mutex> lock(p.mu);
+    for (auto& t : p.pending)
+      if (t.slot == slot_ && t.mark.stream() == stream_.stream()) { t.mark.renew(); return; }
+    p.pending.push_back({slot_, Mark(stream_), true});
+  }
+  int32_t* words = nullptr;
+
+ private:
+  int dev_, slot_;
+  c10::cuda::CUDAStream stream_;
+  Tensor own_;
+  bool captured_;
+};
+
 struct LoraCall {
   Rows x, dy;
+  bool tensor_cores;                                 // decided by types and sizes alone: forward and backward agree
   Tensor w, bias, a, b, scaling, ids;
   tdb::Lora l{};
   LoraCall(const Tensor& x_, const Tensor& w_, const OptTensor& bias_, const Tensor& a_, const Tensor& b_, const OptTensor& scaling_, double scaling_value, const OptTensor& ids_)
-      : x(x_), w(w_.contiguous()), a(a_.contiguous()), b(b_.contiguous()) {
-    l.x = x.ptr(); l.x_stride = x.stride; l.rows = x.rows; l.cols = (int)x.cols;
+      : x(x_), w(rows_of_16_bytes(w_)), a(rows_of_16_bytes(a_)), b(rows_of_16_bytes(b_)) {
+    l.rows = x.rows; l.cols = (int)x.cols;
     l.features = (int)w.size(0); l.rank = (int)a.size(1); l.n = (int)a.size(0); l.dtype = dtype_code(x_);
+    tensor_cores = tdb_lora_umma_applies(&l);
+    fit(x);
+    l.x = x.ptr(); l.x_stride = x.stride;
     l.w = w.data_ptr(); l.a = a.data_ptr(); l.b = b.data_ptr();
-    if (bias_) { bias = bias_->contiguous(); l.bias = bias.data_ptr(); }
+    if (bias_) { bias = rows_of_16_bytes(*bias_); l.bias = bias.data_ptr(); }
     l.scaling_value = (float)scaling_value;
     if (scaling_) { scaling = scaling_->contiguous(); l.scaling = scaling.data_ptr<float>(); }
     l.rows_per_id = 1;
@@ -207,6 +257,19 @@ struct LoraCall {
       if (ids.numel()) l.rows_per_id = l.rows / ids.numel();
     }
   }
+  void set_dy(const Tensor& g) {
+    dy = Rows(g);
+    fit(dy);
+    l.dy = dy.ptr();
+    l.dy_stride = dy.stride;
+  }
+  // Rows that the tensor-core kernels can address.
+  void fit(Rows& r) const {
+    if (tensor_cores && r.rows && (misaligned(r.t) || r.stride % 8 || r.stride < r.cols)) {
+      r.t = rows_of_16_bytes(r.t);
+      r.stride = r.cols;
+    }
+  }
   Tensor floats(at::IntArrayRef sizes) const { return at::empty(sizes, w.options().dtype(at::kFloat)); }
   // The product alone, in fp32.
   Tensor product(const Tensor& left, const Tensor& right) const {
@@ -214,17 +277,47 @@ struct LoraCall {
   }
 };
 
-// h: the adapters' inner values in the form that the gradient of b is made from, where `keep` asks for them.
-std::pair<Tensor, Tensor> run_lora(LoraCall& c, at::IntArrayRef shape, bool keep) {
-  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
-  if (c.l.rows == 0) return {at::empty(shape, c.w.options()), c.floats({1, 0, c.l.rank})};
-  const int shares = tdb_lora_shares(&c.l, 0);
-  Tensor h = c.floats({shares, c.l.rows, c.l.rank});
-  check_rc(tdb_lora_shrink(&c.l, 0, h.data_ptr<float>(), shares, stream));
-  const Tensor base = c.product(c.x.t, c.w.t());
-  Tensor y = c.l.dtype == TDB_DTYPE_F32 ? base : at::empty({c.l.rows, c.l.features}, c.w.options());
-  check_rc(tdb_lora_expand(&c.l, 0, base.data_ptr<float>(), h.data_ptr<float>(), shares, y.data_ptr(), stream));
-  return {y.view(shape), keep ? h : Tensor()};
+// The inner values of the rows: bf16 [rows, inner] from the tensor cores, else fp32 [shares, rows, rank].  f: the factors, for the former.
+Tensor lora_shrink(const LoraCall& c, bool back, const Tensor& f, cudaStream_t stream) {
+  Tensor h;
+  if (c.tensor_cores) {
+    h = at::empty({c.l.rows, tdb_lora_inner(&c.l)}, c.w.options());
+    check_rc(tdb_lora_umma_shrink(&c.l, back, f.data_ptr(), h.data_ptr(), stream));
+  } else {
+    const int shares = tdb_lora_shares(&c.l, back);
+    h = c.floats({shares, c.l.rows, c.l.rank});
+    check_rc(tdb_lora_shrink(&c.l, back, h.data_ptr<float>(), shares, stream));
+  }
+  return h;
+}
+// y [rows, features], or dx [rows, cols], from the rows and their inner values.
+Tensor lora_product(const LoraCall& c, bool back, const Tensor& f, const Tensor& h, c10::cuda::CUDAStream stream) {
+  const int64_t cols = back ? c.l.cols : c.l.features;
+  if (c.tensor_cores) {
+    Tensor y = at::empty({c.l.rows, cols}, c.w.options());
+    StandingReport report(c.w.get_device(), stream);
+    check_rc(tdb_lora_umma_product(&c.l, back, f.data_ptr(), h.data_ptr(), y.data_ptr(), report.words, stream.stream()));
+    report.list();
+    return y;
+  }
+  const Tensor base = back ? c.product(c.dy.t, c.w) : c.product(c.x.t, c.w.t());
+  Tensor y = c.l.dtype == TDB_DTYPE_F32 ? base : at::empty({c.l.rows, cols}, c.w.options());
+  check_rc(tdb_lora_expand(&c.l, back, base.data_ptr<float>(), h.data_ptr<float>(), (int)h.size(0), y.data_ptr(), stream.stream()));
+  return y;
+}
+// [n, r, c] -> [n, c, r]
+Tensor lora_turned(const Tensor& t, cudaStream_t stream) {
+  Tensor out = at::empty({t.size(0), t.size(2), t.size(1)}, t.options());
+  check_rc(tdb_lora_turn(t.data_ptr(), (int)t.size(0), (int)t.size(1), (int)t.size(2), out.data_ptr(), stream));
+  return out;
+}
+
+// y, and the rows' inner values, from which the gradient of b is made.
+std::pair<Tensor, Tensor> run_lora(LoraCall& c, at::IntArrayRef shape) {
+  const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream();
+  if (c.l.rows == 0) return {at::empty(shape, c.w.options()), Tensor()};
+  const Tensor h = lora_shrink(c, false, c.a, stream);
+  return {lora_product(c, false, c.b, h, stream).view(shape), h};
 }
 
 Tensor lora_gradient(const LoraCall& c, bool of_b, const Tensor& v, cudaStream_t stream) {
@@ -232,7 +325,9 @@ Tensor lora_gradient(const LoraCall& c, bool of_b, const Tensor& v, cudaStream_t
   if (c.l.rows == 0) return at::zeros_like(like);
   const int shares = tdb_lora_gather_shares(&c.l, of_b);
   Tensor part = c.floats({shares, c.l.n, c.l.rank, of_b ? c.l.features : c.l.cols}), out = at::empty(like.sizes(), like.options());
-  check_rc(tdb_lora_gather(&c.l, of_b, v.data_ptr<float>(), (int)v.size(0), part.data_ptr<float>(), shares, out.data_ptr(), stream));
+  if (c.tensor_cores) check_rc(tdb_lora_umma_gather(&c.l, of_b, v.data_ptr(), part.data_ptr<float>(), shares, stream));
+  else check_rc(tdb_lora_gather(&c.l, of_b, v.data_ptr<float>(), (int)v.size(0), part.data_ptr<float>(), shares, stream));
+  check_rc(tdb_lora_gather_sum(&c.l, of_b, part.data_ptr<float>(), shares, out.data_ptr(), stream));
   return out;
 }
 
@@ -243,8 +338,8 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
     at::AutoDispatchBelowAutograd below;
     c10::cuda::CUDAGuard guard(x.device());
     LoraCall c(x, w, bias, a, b, scaling, scaling_value, ids);
-    auto [y, h] = run_lora(c, shape, b.requires_grad());
-    ctx->save_for_backward({x, w, a, b, scaling ? *scaling : Tensor(), ids ? *ids : Tensor(), h});
+    auto [y, h] = run_lora(c, shape);
+    ctx->save_for_backward({x, w, a, b, scaling ? *scaling : Tensor(), ids ? *ids : Tensor(), b.requires_grad() ? h : Tensor()});
     ctx->saved_data["scaling"] = scaling_value;
     ctx->saved_data["bias"] = bias.has_value();
     return y;
@@ -256,27 +351,18 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
     const int at = ctx->saved_data["bias"].toBool() ? 3 : 2;
     const bool need_x = ctx->needs_input_grad(0), need_a = ctx->needs_input_grad(at), need_b = ctx->needs_input_grad(at + 1);
     c10::cuda::CUDAGuard guard(x.device());
-    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
+    const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream();
     LoraCall c(x, w, std::nullopt, a, b, scaling.defined() ? OptTensor(scaling) : std::nullopt, ctx->saved_data["scaling"].toDouble(),
                ids.defined() ? OptTensor(ids) : std::nullopt);
-    c.dy = Rows(grads[0]);
-    c.l.dy = c.dy.ptr();
-    c.l.dy_stride = c.dy.stride;
+    c.set_dy(grads[0]);
     Tensor dx, da, db, u;
-    if (c.l.rows && (need_x || need_a)) {
-      const int shares = tdb_lora_shares(&c.l, 1);
-      u = c.floats({shares, c.l.rows, c.l.rank});
-      check_rc(tdb_lora_shrink(&c.l, 1, u.data_ptr<float>(), shares, stream));
-    }
-    if (need_x) {
-      if (c.l.rows == 0) {
-        dx = at::empty(x.sizes(), x.options());
-      } else {
-        const Tensor base = c.product(c.dy.t, c.w);
-        dx = c.l.dtype == TDB_DTYPE_F32 ? base : at::empty({c.l.rows, c.l.cols}, c.w.options());
-        check_rc(tdb_lora_expand(&c.l, 1, base.data_ptr<float>(), u.data_ptr<float>(), (int)u.size(0), dx.data_ptr(), stream));
-        dx = dx.view(x.sizes());
-      }
+    if (c.l.rows == 0) {
+      if (need_x) dx = at::empty(x.sizes(), x.options());
+    } else if (need_x || need_a) {
+      // the product may start beside the kernel in front of it, which therefore is the one that makes u
+      const Tensor a_turned = c.tensor_cores && need_x ? lora_turned(c.a, stream) : Tensor(), b_turned = c.tensor_cores ? lora_turned(c.b, stream) : Tensor();
+      u = lora_shrink(c, true, b_turned, stream);
+      if (need_x) dx = lora_product(c, true, a_turned, u, stream).view(x.sizes());
     }
     if (need_a) da = lora_gradient(c, false, u, stream);
     if (need_b) db = lora_gradient(c, true, h, stream);
@@ -318,5 +404,5 @@ Tensor lora_linear(const Tensor& x, const Tensor& w, const OptTensor& bias, cons
   }
   c10::cuda::CUDAGuard guard(x.device());
   LoraCall c(x, w, bias, a, b, scaling, scaling_value, ids);
-  return run_lora(c, shape, false).first;
+  return run_lora(c, shape).first;
 }

@@ -201,12 +201,16 @@ int expand(const Lora& l, bool back, const float* base, const float* h, int shar
   return cuda_fail(cudaGetLastError(), "lora expand launch");
 }
 template <typename T>
-int gather(const Lora& l, bool of_b, const float* v, int v_shares, float* part, int shares, void* out, cudaStream_t s) {
+int gather(const Lora& l, bool of_b, const float* v, int v_shares, float* part, int shares, cudaStream_t s) {
   const int cols = of_b ? l.features : l.cols, j_blocks = (l.rank + 15) / 16;
   const dim3 grid((cols + COLS - 1) / COLS, l.n * j_blocks, shares);
   gather_kernel<T><<<grid, COLS, 0, s>>>((const T*)(of_b ? l.dy : l.x), of_b ? l.dy_stride : l.x_stride, cols, v, v_shares, l.rank, rows_of(l),
                                          (l.rows + shares - 1) / shares, j_blocks, part);
-  if (const int rc = cuda_fail(cudaGetLastError(), "lora gather launch")) return rc;
+  return cuda_fail(cudaGetLastError(), "lora gather launch");
+}
+template <typename T>
+int gather_sum(const Lora& l, bool of_b, const float* part, int shares, void* out, cudaStream_t s) {
+  const int cols = of_b ? l.features : l.cols;
   const int64_t total = (int64_t)l.n * l.rank * cols;
   const unsigned blocks = (unsigned)((total + 255) / 256);
   if (of_b) gather_sum_kernel<T, true><<<blocks, 256, 0, s>>>(part, shares, total, l.rank, cols, (T*)out);
@@ -244,9 +248,13 @@ int tdb_lora_expand(const Lora* l, int back, const float* base, const float* h, 
   return l->dtype == TDB_DTYPE_F32 ? expand<float>(*l, back, base, h, shares, y, (cudaStream_t)stream)
                                    : expand<__nv_bfloat16>(*l, back, base, h, shares, y, (cudaStream_t)stream);
 }
-int tdb_lora_gather(const Lora* l, int of_b, const float* v, int v_shares, float* part, int shares, void* out, void* stream) {
-  return l->dtype == TDB_DTYPE_F32 ? gather<float>(*l, of_b, v, v_shares, part, shares, out, (cudaStream_t)stream)
-                                   : gather<__nv_bfloat16>(*l, of_b, v, v_shares, part, shares, out, (cudaStream_t)stream);
+int tdb_lora_gather(const Lora* l, int of_b, const float* v, int v_shares, float* part, int shares, void* stream) {
+  return l->dtype == TDB_DTYPE_F32 ? gather<float>(*l, of_b, v, v_shares, part, shares, (cudaStream_t)stream)
+                                   : gather<__nv_bfloat16>(*l, of_b, v, v_shares, part, shares, (cudaStream_t)stream);
+}
+int tdb_lora_gather_sum(const Lora* l, int of_b, const float* part, int shares, void* out, void* stream) {
+  return l->dtype == TDB_DTYPE_F32 ? gather_sum<float>(*l, of_b, part, shares, out, (cudaStream_t)stream)
+                                   : gather_sum<__nv_bfloat16>(*l, of_b, part, shares, out, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -7,7 +7,7 @@
 // add the bias and store bf16 rows.  Bound by HBM traffic: e * (hidden^2 + 2 * two_span * hidden) bytes per call,
 // which at these sizes (a few MB) is a launch-latency-sized kernel.
 #include "tdb_internal.h"
-#include "ptx_sm100.cuh"
+#include "attn_common.cuh"
 #include <cudaTypedefs.h>
 #include <mutex>
 
@@ -154,11 +154,13 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-int map_2d(CUtensorMap* m, const void* ptr, uint64_t cols, uint64_t rows, uint32_t box_rows, const char* what) {
+}  // namespace
+
+int bf16_map_2d(CUtensorMap* m, const void* ptr, uint64_t cols, uint64_t rows, uint64_t stride, uint32_t box_rows, const char* what) {
   auto fn = encode_fn();
   if (!fn) { set_error("cuTensorMapEncodeTiled entry point not found"); return TDB_ERR_CUDA; }
   uint64_t dims[2] = {cols, rows};
-  uint64_t strides[1] = {cols * 2};
+  uint64_t strides[1] = {stride * 2};
   uint32_t box[2] = {PK, box_rows};
   uint32_t estr[2] = {1, 1};
   CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
@@ -167,8 +169,6 @@ int map_2d(CUtensorMap* m, const void* ptr, uint64_t cols, uint64_t rows, uint32
   if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled(%s) failed with CUresult %d", what, (int)r); return TDB_ERR_CUDA; }
   return TDB_OK;
 }
-
-}  // namespace
 
 // True when the tensor-core kernel applies: bf16, head_dim 64, rows of 16-byte multiples, 16-byte aligned bases.
 bool relpos_umma_applicable(const void* rel, const void* W, const void* out, int hidden, int D, int dtype) {
@@ -180,8 +180,8 @@ int launch_relpos_project_umma(const void* rel, const void* W, const void* bias,
                                void* out, int32_t* status, cudaStream_t s) {
   CUtensorMap tm_rel, tm_w;
   int rc;
-  if ((rc = map_2d(&tm_rel, rel, (uint64_t)hidden, (uint64_t)two_span, PM, "rel"))) return rc;
-  if ((rc = map_2d(&tm_w, W, (uint64_t)hidden, (uint64_t)H * PN, PN, "W"))) return rc;
+  if ((rc = bf16_map_2d(&tm_rel, rel, (uint64_t)hidden, (uint64_t)two_span, (uint64_t)hidden, PM, "rel"))) return rc;
+  if ((rc = bf16_map_2d(&tm_w, W, (uint64_t)hidden, (uint64_t)H * PN, (uint64_t)hidden, PN, "W"))) return rc;
   if ((rc = opt_in_smem(reinterpret_cast<const void*>(relpos_project_umma_kernel), (int)P_SMEM))) return rc;
   dim3 grid((two_span + PM - 1) / PM, H);
   relpos_project_umma_kernel<<<grid, P_THREADS, P_SMEM, s>>>(tm_rel, tm_w, (const __nv_bfloat16*)bias, two_span, hidden, H,

@@ -202,5 +202,16 @@ TDB_HOST_API int tdb_lora_shrink(const tdb::Lora* l, int back, float* h, int sha
 TDB_HOST_API int tdb_lora_expand(const tdb::Lora* l, int back, const float* base, const float* h, int shares, void* y, void* stream);
 // The gradient of a (from v = u and x) or of b (from v = h and dy).  part: [shares, n, rank, columns] floats.
 TDB_HOST_API int tdb_lora_gather_shares(const tdb::Lora* l, int of_b);
-TDB_HOST_API int tdb_lora_gather(const tdb::Lora* l, int of_b, const float* v, int v_shares, float* part, int shares, void* out, void* stream);
+TDB_HOST_API int tdb_lora_gather(const tdb::Lora* l, int of_b, const float* v, int v_shares, float* part, int shares, void* stream);
+// The sum of gather's shares, to the type and layout of a (or of b).
+TDB_HOST_API int tdb_lora_gather_sum(const tdb::Lora* l, int of_b, const float* part, int shares, void* out, void* stream);
+// The same on the tensor cores (lora_umma.cu), for bf16 with columns and features that are multiples of eight, all tensors 16-byte aligned and rows no
+// less than a row apart.  f: the factors that are multiplied with x (a) or dy (b turned, [n, rank, features]) in `shrink`, and those that make y (b) or dx (a
+// turned, [n, cols, rank]) in `product`.  hx, v: bf16 [rows, tdb_lora_inner()].  status: int32[4], word 0 tells of a wait that gave up.
+TDB_HOST_API int tdb_lora_umma_applies(const tdb::Lora* l);
+TDB_HOST_API int64_t tdb_lora_inner(const tdb::Lora* l);
+TDB_HOST_API int tdb_lora_umma_shrink(const tdb::Lora* l, int back, const void* f, void* hx, void* stream);
+TDB_HOST_API int tdb_lora_umma_product(const tdb::Lora* l, int back, const void* f, const void* hx, void* y, int32_t* status, void* stream);
+TDB_HOST_API int tdb_lora_umma_gather(const tdb::Lora* l, int of_b, const void* v, float* part, int shares, void* stream);
+TDB_HOST_API int tdb_lora_turn(const void* in, int n, int rows, int cols, void* out, void* stream);
 }
