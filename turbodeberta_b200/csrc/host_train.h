@@ -45,6 +45,7 @@ void check_seed(const OptTensor& seed, const Tensor& x) {
 
 Tensor run_dropout(const Tensor& x, const tdb::Dropout& d) {
   c10::cuda::CUDAGuard guard(x.device());
+  if (d.drop == 0) return x.clone(at::MemoryFormat::Contiguous);
   const Tensor in = x.contiguous();
   Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
   check_rc(tdb_dropout(in.data_ptr(), y.data_ptr(), in.numel(), dtype_code(x), &d, c10::cuda::getCurrentCUDAStream().stream()));

@@ -42,18 +42,16 @@ __device__ __forceinline__ uint4 dropout_bits(uint64_t first, uint64_t offset, u
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Which of eight elements stay, a bit each.
-__device__ __forceinline__ uint32_t staying(const uint4& bits, uint32_t drop) {
+// What stays of eight elements, scaled.  A dropped element is zero whatever it held (NaN and infinities too).
+// drop > 0; above = (drop << 16) - 1: a number is at least `drop` when, in a word's upper half, the word is greater than that.
+__device__ __forceinline__ uint32_t dropout_above(uint32_t drop) { return (drop << 16) - 1; }
+__device__ __forceinline__ void drop8(float* f, const uint4& bits, uint32_t above, float scale) {
   const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
-  uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m |= ((w[i] & 0xffffu) >= drop ? 1u << (2 * i) : 0u) | ((w[i] >> 16) >= drop ? 2u << (2 * i) : 0u);
-  return m;
-}
-// A dropped element is zero whatever it held (NaN and infinities too).
-__device__ __forceinline__ void drop8(float* f, uint32_t stay, float scale) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = stay >> i & 1 ? f[i] * scale : 0.f;
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = w[i] << 16 > above ? f[2 * i] * scale : 0.f;
+    f[2 * i + 1] = w[i] > above ? f[2 * i + 1] * scale : 0.f;
+  }
 }
 
 }  // namespace tdb

@@ -5,9 +5,12 @@
 // Everything works on units of eight consecutive columns: a 16-byte load in bf16, two in fp32, and one block of random bits.
 // VEC: the rows allow that (columns a multiple of eight, aligned rows); otherwise a unit is read element by element.
 #include "tdb_internal.h"
+#include "ptx_sm100.cuh"
 #include "philox.cuh"
+#include <algorithm>
 
 namespace tdb {
+using namespace ptx;
 
 namespace {
 
@@ -30,20 +33,43 @@ __device__ __forceinline__ Unit<T> load_unit(const T* p, int have) {
   }
   return u;
 }
-__device__ __forceinline__ void unpack(const Unit<float>& u, float* f) {
+// Eight elements as four pairs: two fp32 operations go by in one instruction, which is what keeps the kernels below bound by memory.
+struct Eight {
+  f32x2 v[4];
+  __device__ __forceinline__ void unpack(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float2 h = halves(v[i]); f[2 * i] = h.x; f[2 * i + 1] = h.y; }
+  }
+  __device__ __forceinline__ void pack(const float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = pair(f[2 * i], f[2 * i + 1]);
+  }
+};
+__device__ __forceinline__ f32x2 twice(float x) { return pair(x, x); }
+__device__ __forceinline__ f32x2 times(f32x2 a, f32x2 b) { mul2(a, b); return a; }
+__device__ __forceinline__ f32x2 plus(f32x2 a, f32x2 b) { add2(a, b); return a; }
+__device__ __forceinline__ f32x2 fused(f32x2 a, f32x2 b, f32x2 c) { fma2(c, a, b); return c; }
+
+__device__ __forceinline__ Eight eight(const Unit<float>& u) {
+  Eight e;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    f[4 * i] = __uint_as_float(u.v[i].x); f[4 * i + 1] = __uint_as_float(u.v[i].y);
-    f[4 * i + 2] = __uint_as_float(u.v[i].z); f[4 * i + 3] = __uint_as_float(u.v[i].w);
+    e.v[2 * i] = pair(__uint_as_float(u.v[i].x), __uint_as_float(u.v[i].y));
+    e.v[2 * i + 1] = pair(__uint_as_float(u.v[i].z), __uint_as_float(u.v[i].w));
   }
+  return e;
 }
-__device__ __forceinline__ void unpack(const Unit<__nv_bfloat16>& u, float* f) {
+__device__ __forceinline__ Eight eight(const Unit<__nv_bfloat16>& u) {
   const uint32_t w[4] = {u.v[0].x, u.v[0].y, u.v[0].z, u.v[0].w};
+  Eight e;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  for (int i = 0; i < 4; ++i) e.v[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  return e;
 }
 template <bool VEC>
-__device__ __forceinline__ void store_unit(float* p, const float* f, int have) {
+__device__ __forceinline__ void store_unit(float* p, const Eight& x, int have) {
+  float f[8];
+  x.unpack(f);
   if (VEC) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -54,25 +80,26 @@ __device__ __forceinline__ void store_unit(float* p, const float* f, int have) {
   }
 }
 template <bool VEC>
-__device__ __forceinline__ void store_unit(__nv_bfloat16* p, const float* f, int have) {
+__device__ __forceinline__ void store_unit(__nv_bfloat16* p, const Eight& x, int have) {
+  float f[8];
+  x.unpack(f);
   if (VEC) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 t = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&t);
-    }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) if (i < have) p[i] = __float2bfloat16_rn(f[i]);
   }
 }
 // Eight weights of either type.
-__device__ __forceinline__ void load_weights(const void* w, int f32, int64_t at, int have, float* f) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    f[i] = i < have ? (f32 ? static_cast<const float*>(w)[at + i] : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[at + i])) : 0.f;
+template <bool VEC>
+__device__ __forceinline__ Eight load_weights(const void* w, int f32, int at, int have) {
+  return f32 ? eight(load_unit<float, VEC>(static_cast<const float*>(w) + at, have)) : eight(load_unit<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(w) + at, have));
+}
+__device__ __forceinline__ void drop8(Eight& x, const uint4& bits, uint32_t above, float scale) {
+  float f[8];
+  x.unpack(f);
+  tdb::drop8(f, bits, above, scale);
+  x.pack(f);
 }
 
 // ------------------------------------------------------------------------------------------------------------------ dropout
@@ -94,9 +121,8 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, T
     const int64_t at = first + 256 * i;
     if (at >= units) break;
     const int have = (int)min((int64_t)8, n - at * 8);
-    float f[8];
-    unpack(u[i], f);
-    drop8(f, staying(philox((uint64_t)at, (uint64_t)key.offset, seed), key.drop), key.scale);
+    Eight f = eight(u[i]);
+    drop8(f, philox((uint64_t)at, (uint64_t)key.offset, seed), dropout_above(key.drop), key.scale);
     if (VEC && have == 8) store_unit<true>(y + at * 8, f, 8);
     else store_unit<false>(y + at * 8, f, have);
   }
@@ -106,18 +132,41 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, T
 // The threads that share a row are `group` threads of the block (whole warps); sums over them, in a fixed order.
 struct Group {
   int threads, lane, index;               // index: which of the block's groups
-  float* shared;                          // 2 buffers of 32 floats for every value that is summed at once
+  float* shared;                          // two buffers of N floats for every warp of the block
   int flip;
 };
-__device__ __forceinline__ float warp_sum(float x) {
+// Every lane gets the warp's sum of each of N values (1, 2 or 4).  Lanes trade values on the way, so that N sums take N - 1 exchanges more than
+// one, and not five times as many.
+template <int N>
+__device__ __forceinline__ void warp_sums(float* v) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (N == 4) {
+    const bool up = lane & 16;
+    const float a = __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], 16), b = __shfl_xor_sync(0xffffffffu, up ? v[1] : v[3], 16);
+    float w[2] = {(up ? v[2] : v[0]) + a, (up ? v[3] : v[1]) + b};
+    const bool odd = lane & 8;
+    const float c = __shfl_xor_sync(0xffffffffu, odd ? w[0] : w[1], 8);
+    float s = (odd ? w[1] : w[0]) + c;
 #pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-  return x;
+    for (int off = 4; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __shfl_sync(0xffffffffu, s, 8 * i);
+  } else if constexpr (N == 2) {
+    const bool up = lane & 16;
+    const float a = __shfl_xor_sync(0xffffffffu, up ? v[0] : v[1], 16);
+    float s = (up ? v[1] : v[0]) + a;
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    v[0] = __shfl_sync(0xffffffffu, s, 0);
+    v[1] = __shfl_sync(0xffffffffu, s, 16);
+  } else {
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
+  }
 }
 template <int N>
 __device__ __forceinline__ void group_sum(Group& g, float* v) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+  warp_sums<N>(v);
   if (g.threads == 32) return;
   const int warps = g.threads / 32;
   // two buffers in turn: a warp that runs ahead writes the other one, and cannot come round again before the next barrier
@@ -125,14 +174,15 @@ __device__ __forceinline__ void group_sum(Group& g, float* v) {
   g.flip ^= 1;
   if (g.lane % 32 == 0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) buf[i * warps + g.lane / 32] = v[i];
+    for (int i = 0; i < N; ++i) buf[g.lane / 32 * N + i] = v[i];
   }
   asm volatile("bar.sync %0, %1;" ::"r"(g.index + 1), "r"(g.threads) : "memory");
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float s = 0.f;
-    for (int w = 0; w < warps; ++w) s += buf[i * warps + w];
-    v[i] = s;
+  for (int i = 0; i < N; ++i) v[i] = 0.f;
+#pragma unroll 4
+  for (int w = 0; w < warps; ++w) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += buf[w * N + i];
   }
 }
 
@@ -143,26 +193,35 @@ struct NormParams : Norm {
   int group, w_f32;                                         // threads of a row
 };
 
+// Eight elements of what the norm is taken of; `bits` are those that dropped them.
 template <typename T, bool VEC, int MODE>
-__device__ __forceinline__ void joined(const NormParams& p, const Unit<T>& x, const Unit<T>& r, int64_t row, int col, uint64_t seed, float* f, uint32_t& stay) {
-  unpack(x, f);
+__device__ __forceinline__ Eight joined(const NormParams& p, const Unit<T>& x, const Unit<T>& r, int64_t row, int col, uint64_t seed, uint4& bits) {
+  Eight f = eight(x);
   if (MODE == JOIN_DROP) {
-    stay = staying(dropout_bits<VEC>((uint64_t)row * p.cols + col, (uint64_t)p.drop.offset, seed), p.drop.drop);
-    drop8(f, stay, p.drop.scale);
+    bits = dropout_bits<VEC>((uint64_t)row * p.cols + col, (uint64_t)p.drop.offset, seed);
+    drop8(f, bits, dropout_above(p.drop.drop), p.drop.scale);
   }
   if (MODE != ALONE) {
-    float g[8];
-    unpack(r, g);
+    const Eight g = eight(r);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] += g[e];
+    for (int e = 0; e < 4; ++e) add2(f.v[e], g.v[e]);
   }
+  return f;
+}
+// Elements behind the last column become zero.
+__device__ __forceinline__ void cut(Eight& x, int have) {
+  float f[8];
+  x.unpack(f);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = e < have ? f[e] : 0.f;
+  x.pack(f);
 }
 
 // One group of threads to a row, the row in registers; mean first, then the deviations from it (the sum of squares alone would lose
 // the variance of rows far from zero).
 template <typename T, bool VEC, int MODE, int U>
 __global__ void __launch_bounds__(512) norm_forward_kernel(const NormParams p) {
-  extern __shared__ float shared[];
+  extern __shared__ __align__(16) float shared[];
   Group g{p.group, (int)threadIdx.x % p.group, (int)threadIdx.x / p.group, shared, 0};
   const int groups = blockDim.x / p.group;
   const int64_t row = (int64_t)blockIdx.x * groups + g.index;
@@ -179,137 +238,200 @@ __global__ void __launch_bounds__(512) norm_forward_kernel(const NormParams p) {
       if (MODE != ALONE) ru[i] = load_unit<T, VEC>(res + c * 8, p.cols - c * 8);
     }
   }
-  float f[U][8], sum = 0.f;
+  Eight f[U];
+  f32x2 sums = twice(0.f);
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const int c = g.lane + p.group * i;
     if (c < units) {
-      uint32_t stay;
-      joined<T, VEC, MODE>(p, xu[i], ru[MODE == ALONE ? 0 : i], row, c * 8, seed, f[i], stay);
+      uint4 bits;
+      f[i] = joined<T, VEC, MODE>(p, xu[i], ru[MODE == ALONE ? 0 : i], row, c * 8, seed, bits);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += VEC || c * 8 + e < p.cols ? f[i][e] : 0.f;
+      for (int e = 0; e < 4; ++e) add2(sums, f[i].v[e]);     // zeros behind the last column
     }
   }
+  float sum = halves(sums).x + halves(sums).y;
   group_sum<1>(g, &sum);
-  const float mean = sum / (float)p.cols;
-  float sq = 0.f;
+  const f32x2 mean = twice(sum / (float)p.cols), minus = twice(-halves(mean).x);
+  f32x2 squares = twice(0.f);
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const int c = g.lane + p.group * i;
     if (c < units) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        f[i][e] -= mean;
-        sq = VEC || c * 8 + e < p.cols ? fmaf(f[i][e], f[i][e], sq) : sq;
-      }
+      for (int e = 0; e < 4; ++e) add2(f[i].v[e], minus);
+      if (!VEC) cut(f[i], p.cols - c * 8);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) fma2(squares, f[i].v[e], f[i].v[e]);
     }
   }
+  float sq = halves(squares).x + halves(squares).y;
   group_sum<1>(g, &sq);
   const float inv = rsqrtf(sq / (float)p.cols + p.eps);
-  if (p.stats && g.lane == 0) *reinterpret_cast<float2*>(p.stats + 2 * row) = make_float2(mean, inv);
+  if (p.stats && g.lane == 0) *reinterpret_cast<float2*>(p.stats + 2 * row) = make_float2(halves(mean).x, inv);
+  const f32x2 scale = twice(inv);
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const int c = g.lane + p.group * i;
     if (c < units) {
-      float w[8], b[8];
-      load_weights(p.w, p.w_f32, c * 8, p.cols - c * 8, w);
-      load_weights(p.b, p.w_f32, c * 8, p.cols - c * 8, b);
+      const Eight w = load_weights<VEC>(p.w, p.w_f32, c * 8, p.cols - c * 8), b = load_weights<VEC>(p.b, p.w_f32, c * 8, p.cols - c * 8);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[i][e] = fmaf(f[i][e] * inv, w[e], b[e]);
+      for (int e = 0; e < 4; ++e) f[i].v[e] = fused(times(f[i].v[e], scale), w.v[e], b.v[e]);
       store_unit<VEC>((T*)p.y + row * p.cols + c * 8, f[i], p.cols - c * 8);
     }
   }
 }
 
 // Backward.  With g = dy w and h = (z - mean) inv:  dz = (g - mean(g) - h mean(g h)) inv, dw = sum over rows of dy h, db of dy.
-// A group of threads keeps the same columns for all its rows, so the weights and both column sums stay in registers; R rows are in
-// flight at once, and their 2 R sums share one exchange.  The sums of a block go to `partial` and are added up by the kernel behind
-// this one, in a fixed order: atomics would make two runs differ.
+// A group of threads keeps the same columns for all its rows, so the weights and both column sums stay in registers, and the 2 R sums of
+// the R rows that it takes at once share one exchange.  A block's sums go to `partial` and are added up by the kernel behind this one, in a
+// fixed order: atomics would make two runs differ.
+// VEC: what a thread will read is on its way several rounds ahead, by asynchronous copies into shared memory that no other thread touches:
+// an SM has some 150 KB in flight while it computes, without barriers or registers for it.
+constexpr int RING_BYTES = 192 * 1024;
+template <typename T, int MODE, int U, int R>
+__host__ __device__ constexpr int round_bytes() { return R * U * (MODE == ALONE ? 2 : 3) * (int)sizeof(Unit<T>); }     // of one thread
+template <typename T, int MODE, int U, int R>
+__host__ __device__ constexpr int rounds_ahead() { return RING_BYTES / 512 / round_bytes<T, MODE, U, R>() < 4 ? RING_BYTES / 512 / round_bytes<T, MODE, U, R>() : 4; }
+
 template <typename T, bool VEC, int MODE, int U, int R>
 __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormParams p) {
-  extern __shared__ float shared[];
-  Group g{p.group, (int)threadIdx.x % p.group, (int)threadIdx.x / p.group, shared, 0};
+  extern __shared__ __align__(16) float shared[];
+  constexpr int STAGES = VEC ? rounds_ahead<T, MODE, U, R>() : 0, NT = MODE == ALONE ? 2 : 3, PIECES = (int)sizeof(Unit<T>) / 16;
+  float* ring = shared;
+  float* exchange = shared + STAGES * round_bytes<T, MODE, U, R>() / 4 * blockDim.x;
+  Group g{p.group, (int)threadIdx.x % p.group, (int)threadIdx.x / p.group, exchange, 0};
   const int groups = blockDim.x / p.group, units = (p.cols + 7) / 8;
   const uint64_t seed = MODE == JOIN_DROP ? dropout_seed(p.drop) : 0;
-  float w[U][8], dw[U][8], db[U][8];
+  const uint32_t above = dropout_above(p.drop.drop);
+  Eight w[U], dw[U], db[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const int c = g.lane + p.group * i;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[i][e] = dw[i][e] = db[i][e] = 0.f;
-    if (c < units) load_weights(p.w, p.w_f32, c * 8, p.cols - c * 8, w[i]);
+    for (int e = 0; e < 4; ++e) w[i].v[e] = dw[i].v[e] = db[i].v[e] = twice(0.f);
+    if (c < units) w[i] = load_weights<VEC>(p.w, p.w_f32, c * 8, p.cols - c * 8);
   }
   const float over = 1.f / (float)p.cols;
-  for (int64_t row0 = ((int64_t)blockIdx.x * groups + g.index) * R; row0 < p.rows; row0 += (int64_t)gridDim.x * groups * R) {
-    Unit<T> xu[R][U], ru[MODE == ALONE ? 1 : R][U], du[R][U];
-    float2 st[R];
+  const int64_t first = ((int64_t)blockIdx.x * groups + g.index) * R, stride = (int64_t)gridDim.x * groups * R;
+  // tensor k of x, residual, dy
+  auto source = [&](int k, int64_t row, int c) {
+    return k == 0 ? (const T*)p.x + row * p.x_stride + c * 8 : k == NT - 1 ? (const T*)p.dy + row * p.dy_stride + c * 8 : (const T*)p.res + row * p.res_stride + c * 8;
+  };
+  const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16, pitch = blockDim.x * 16;
+  const uint32_t stage_bytes = NT * R * U * PIECES * pitch;
+  auto slot = [&](uint32_t stage, int k, int r, int i, int piece) { return stage + (uint32_t)(((k * R + r) * U + i) * PIECES + piece) * pitch; };
+  auto ask = [&](int64_t row0, uint32_t stage) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t row = min(row0 + r, p.rows - 1);        // a row behind the last one is the last one again, and counts for nothing
-      st[r] = *reinterpret_cast<const float2*>(p.stats + 2 * row);
+      if (row0 + r >= p.rows) break;
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int c = g.lane + p.group * i;
-        if (c < units) {
-          xu[r][i] = load_unit<T, VEC>((const T*)p.x + row * p.x_stride + c * 8, p.cols - c * 8);
-          if (MODE != ALONE) ru[r][i] = load_unit<T, VEC>((const T*)p.res + row * p.res_stride + c * 8, p.cols - c * 8);
-          du[r][i] = load_unit<T, VEC>((const T*)p.dy + row * p.dy_stride + c * 8, p.cols - c * 8);
-        }
+      for (int k = 0; k < NT; ++k) {
+        const T* row = source(k, row0 + r, g.lane);
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+          if (g.lane + p.group * i < units) {
+#pragma unroll
+            for (int piece = 0; piece < PIECES; ++piece)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot(stage, k, r, i, piece)),
+                           "l"(reinterpret_cast<const uint4*>(row + p.group * i * 8) + piece) : "memory");
+          }
       }
     }
-    float h[R][U][8], sums[2 * R];
-    uint32_t stay[R][U];
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto unit = [&](uint32_t stage, int k, int64_t row, int r, int i) {
+    const int c = g.lane + p.group * i;
+    Unit<T> u;
+    if constexpr (VEC) {
+#pragma unroll
+      for (int piece = 0; piece < PIECES; ++piece) {
+        uint4& v = u.v[piece];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(slot(stage, k, r, i, piece)) : "memory");
+      }
+    } else {
+      u = load_unit<T, false>(source(k, row, c), p.cols - c * 8);
+    }
+    return u;
+  };
+  auto stat = [&](int64_t row) { return *reinterpret_cast<const float2*>(p.stats + 2 * (row < p.rows ? row : p.rows - 1)); };
+  if constexpr (VEC) {
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) ask(first + s * stride, mine + s * stage_bytes);
+  }
+  float2 soon[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) soon[r] = stat(first + r);
+  uint32_t stage = mine, before = mine + (VEC ? STAGES - 1 : 0) * stage_bytes;      // of this round, and of the one before it
+  for (int64_t row0 = first; row0 < p.rows; row0 += stride) {
+    if constexpr (VEC) {
+      ask(row0 + (STAGES - 1) * stride, before);
+      asm volatile("cp.async.wait_group %0;" ::"n"(VEC ? STAGES - 1 : 0) : "memory");
+    }
+    float2 st[R];
+    Eight h[R][U];
+    float sums[2 * R];
+    uint4 bits[R][U];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const bool real = row0 + r < p.rows;
+      st[r] = soon[r];
+      soon[r] = stat(row0 + stride + r);
+      f32x2 s1 = twice(0.f), s2 = twice(0.f);
       sums[2 * r] = sums[2 * r + 1] = 0.f;
+      if (row0 + r >= p.rows) continue;
+      const f32x2 minus = twice(-st[r].x), inv = twice(st[r].y);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int c = g.lane + p.group * i;
         if (c >= units) continue;
-        joined<T, VEC, MODE>(p, xu[r][i], ru[MODE == ALONE ? 0 : r][i], row0 + r, c * 8, seed, h[r][i], stay[r][i]);
-        float d[8];
-        unpack(du[r][i], d);
+        const Unit<T> xu = unit(stage, 0, row0 + r, r, i);
+        h[r][i] = joined<T, VEC, MODE>(p, xu, MODE == ALONE ? xu : unit(stage, 1, row0 + r, r, i), row0 + r, c * 8, seed, bits[r][i]);
+        const Eight d = eight(unit(stage, NT - 1, row0 + r, r, i));          // zeros behind the last column, and in w too
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool in = real && (VEC || c * 8 + e < p.cols);
-          h[r][i][e] = (h[r][i][e] - st[r].x) * st[r].y;
-          dw[i][e] = in ? fmaf(d[e], h[r][i][e], dw[i][e]) : dw[i][e];
-          db[i][e] = in ? db[i][e] + d[e] : db[i][e];
-          const float gw = d[e] * w[i][e];                  // zero behind the last column
-          sums[2 * r] += VEC || in ? gw : 0.f;
-          sums[2 * r + 1] = VEC || in ? fmaf(gw, h[r][i][e], sums[2 * r + 1]) : sums[2 * r + 1];
+        for (int e = 0; e < 4; ++e) h[r][i].v[e] = times(plus(h[r][i].v[e], minus), inv);
+        if (!VEC) cut(h[r][i], p.cols - c * 8);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          fma2(dw[i].v[e], d.v[e], h[r][i].v[e]);
+          add2(db[i].v[e], d.v[e]);
+          const f32x2 gw = times(d.v[e], w[i].v[e]);
+          add2(s1, gw);
+          fma2(s2, gw, h[r][i].v[e]);
         }
       }
+      sums[2 * r] = halves(s1).x + halves(s1).y;
+      sums[2 * r + 1] = halves(s2).x + halves(s2).y;
     }
     group_sum<2 * R>(g, sums);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int64_t row = row0 + r;
       if (row >= p.rows) break;
-      const float c1 = sums[2 * r] * over, c2 = sums[2 * r + 1] * over;
+      const f32x2 c1 = twice(-sums[2 * r] * over), c2 = twice(-sums[2 * r + 1] * over), inv = twice(st[r].y);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int c = g.lane + p.group * i;
         if (c >= units) continue;
-        float d[8];
-        unpack(du[r][i], d);
+        Eight d = eight(unit(stage, NT - 1, row, r, i));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = (fmaf(d[e], w[i][e], -c1) - h[r][i][e] * c2) * st[r].y;
+        for (int e = 0; e < 4; ++e) d.v[e] = times(fused(h[r][i].v[e], c2, fused(d.v[e], w[i].v[e], c1)), inv);
         const int64_t at = row * p.cols + c * 8;
         if (MODE == ALONE && p.dx) store_unit<VEC>((T*)p.dx + at, d, p.cols - c * 8);
         if (MODE != ALONE && p.dres) store_unit<VEC>((T*)p.dres + at, d, p.cols - c * 8);
         if (MODE == JOIN_DROP && p.dx) {
-          drop8(d, stay[r][i], p.drop.scale);
+          drop8(d, bits[r][i], above, p.drop.scale);
           store_unit<VEC>((T*)p.dx + at, d, p.cols - c * 8);
         }
       }
     }
+    before = stage;
+    if constexpr (VEC) stage = stage + stage_bytes == mine + STAGES * stage_bytes ? mine : stage + stage_bytes;
   }
   let_next_start();
   if (!p.partial) return;
-  // the block's groups add up their column sums, one after the other
-  float* sum = shared + (p.group == 32 ? 0 : groups * 2 * 2 * R * (p.group / 32));
+  // the block's groups add up their column sums, one after the other, where the ring was
+  if constexpr (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  float* sum = shared;
   for (int k = 0; k < groups; ++k) {
     __syncthreads();
     if (g.index != k) continue;
@@ -321,8 +443,9 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormParams 
       for (int e = 0; e < 8; ++e) {
         float* a = sum + e * units + c;                     // by element, so that neighbouring threads meet different banks
         float* b = a + 8 * units;
-        *a = k ? *a + dw[i][e] : dw[i][e];
-        *b = k ? *b + db[i][e] : db[i][e];
+        const float2 w2 = halves(dw[i].v[e / 2]), b2 = halves(db[i].v[e / 2]);
+        *a = (k ? *a : 0.f) + (e % 2 ? w2.y : w2.x);
+        *b = (k ? *b : 0.f) + (e % 2 ? b2.y : b2.x);
       }
     }
   }
@@ -365,9 +488,9 @@ int norm_forward(NormParams p, cudaStream_t s) {
   if (const int rc = device_sms(&sms)) return rc;
   auto run = [&](auto kernel, int u) {
     p.group = group_threads(units, u);
-    const int groups = p.rows >= 16 * sms ? max(1, 128 / p.group) : 1;      // few rows: one per block, so that they spread over the SMs
+    const int groups = p.rows >= 16 * sms ? max(1, 256 / p.group) : 1;      // few rows: one per block, so that they spread over the SMs
     const int64_t blocks = (p.rows + groups - 1) / groups;
-    kernel<<<(unsigned)blocks, groups * p.group, groups * 2 * (p.group / 32) * sizeof(float), s>>>(p);
+    kernel<<<(unsigned)blocks, groups * p.group, p.group == 32 ? 0 : groups * 2 * (p.group / 32) * sizeof(float), s>>>(p);
     return cuda_fail(cudaGetLastError(), "norm launch");
   };
   if (units <= 32) return run(norm_forward_kernel<T, VEC, MODE, 1>, 1);
@@ -396,24 +519,26 @@ BackwardShape backward_shape(int64_t rows, int cols, int most_rows, int sms) {
 
 template <typename T, bool VEC, int MODE>
 int norm_backward(NormParams p, cudaStream_t s) {
-  constexpr int R = !VEC ? 1 : sizeof(T) == 2 ? 4 : 2;       // what the registers hold
+  constexpr int R = VEC && sizeof(T) == 2 ? 2 : 1;
   int sms = 0, rc;
   if ((rc = device_sms(&sms))) return rc;
   const BackwardShape b = backward_shape(p.rows, p.cols, R, sms);
   const int units = (p.cols + 7) / 8;
   p.group = b.group;
-  auto run = [&](auto kernel, int r) -> int {
-    const int exchange = b.group == 32 ? 0 : b.groups * 2 * 2 * r * (b.group / 32);
-    const int bytes = (exchange + (p.partial ? 16 * units : 0)) * (int)sizeof(float);
+  auto run = [&](auto kernel, int r, int ring) -> int {       // ring: bytes of one thread
+    const int exchange = b.group == 32 ? 0 : b.groups * 2 * 2 * r * (b.group / 32) * 4, threads = b.groups * b.group;
+    const int bytes = std::max(VEC ? ring * threads + exchange : exchange, (VEC ? 0 : exchange) + (p.partial ? 16 * units * 4 : 0));
     if (bytes > 48 * 1024)
       if (const int rc = opt_in_smem(reinterpret_cast<const void*>(kernel), 227 * 1024)) return rc;
-    kernel<<<b.blocks, b.groups * b.group, bytes, s>>>(p);
+    kernel<<<b.blocks, threads, bytes, s>>>(p);
     return cuda_fail(cudaGetLastError(), "norm backward launch");
   };
-  if (b.rows_each == R && R > 1) rc = run(norm_backward_kernel<T, VEC, MODE, 1, R>, R);
-  else if (b.units_each == 1) rc = run(norm_backward_kernel<T, VEC, MODE, 1, 1>, 1);
-  else if (b.units_each == 2) rc = run(norm_backward_kernel<T, VEC, MODE, 2, 1>, 1);
-  else rc = run(norm_backward_kernel<T, VEC, MODE, 4, 1>, 1);
+#define TDB_BACKWARD(U, R) run(norm_backward_kernel<T, VEC, MODE, U, R>, R, rounds_ahead<T, MODE, U, R>() * round_bytes<T, MODE, U, R>())
+  if (b.rows_each == R && R > 1) rc = TDB_BACKWARD(1, R);
+  else if (b.units_each == 1) rc = TDB_BACKWARD(1, 1);
+  else if (b.units_each == 2) rc = TDB_BACKWARD(2, 1);
+  else rc = TDB_BACKWARD(4, 1);
+#undef TDB_BACKWARD
   if (rc || !p.partial) return rc;
   return cuda_fail(launch_early(norm_weights_kernel, dim3((2 * p.cols + 31) / 32), 512, 0, s, (const float*)p.partial, b.blocks, p.cols, p.w_f32, p.dw, p.db),
                    "norm weights launch");
@@ -425,7 +550,7 @@ template <typename T>
 bool vectors(const NormParams& p) {
   const int per = 16 / (int)sizeof(T);
   return p.cols % 8 == 0 && p.x_stride % per == 0 && p.res_stride % per == 0 && p.dy_stride % per == 0 && aligned(p.x) && aligned(p.res) &&
-         aligned(p.dy) && aligned(p.y) && aligned(p.dx) && aligned(p.dres);
+         aligned(p.dy) && aligned(p.y) && aligned(p.dx) && aligned(p.dres) && aligned(p.w) && aligned(p.b);
 }
 
 template <typename T>
