@@ -21,14 +21,16 @@ namespace {
 using bf16 = __nv_bfloat16;
 
 // Goes through the adapters of 32 N rows, each once, in the order of their first rows; a whole warp holds the ids, lane l those of
-// rows l, l + 32, ...
+// rows l, l + 32, ...  load() only asks for them, so that their way from memory can pass beside other work.
 template <int N>
 struct Adapters {
   int id[N];
   uint32_t left[N];
-  __device__ __forceinline__ Adapters(const LoraRows& rows, int64_t t0, int lane) {
+  __device__ __forceinline__ void load(const LoraRows& rows, int64_t t0, int lane) {
 #pragma unroll
     for (int i = 0; i < N; ++i) id[i] = t0 + 32 * i + lane < rows.rows ? adapter_of(rows, t0 + 32 * i + lane) : -1;
+  }
+  __device__ __forceinline__ void start() {
 #pragma unroll
     for (int i = 0; i < N; ++i) left[i] = __ballot_sync(0xffffffffu, id[i] >= 0);
   }
@@ -44,7 +46,8 @@ struct Adapters {
     }
     return a;
   }
-  __device__ __forceinline__ int count() {              // goes through them
+  __device__ __forceinline__ int count() {
+    start();
     int n = 0;
     while (next() >= 0) ++n;
     return n;
@@ -52,30 +55,50 @@ struct Adapters {
 };
 
 // ------------------------------------------------------------------------------------------------------------------- shrink
-// hx[t] = the inner values of row t: r16 high parts, r16 low parts.  A block: 16 MT rows and 8 NJ factors; its eight warps share the columns,
-// blocks of 32 in turn, and add up through shared memory.  Bound by reading x, and the factors from L2 once for every block.  As in the skinny
-// projections a thread's fragments of two k16 steps are one 16-byte load, since the order of the columns inside a product is free.
+// hx[t] = the inner values of row t: r16 high parts, r16 low parts.  A block: 16 MT rows and 8 NJ factors; its warps share the columns, blocks of
+// 64 in turn, and add up through shared memory.  Bound by reading x, and the factors from L2 once for every block: each warp has STAGES blocks
+// of columns on their way into shared memory that is its own, so that nothing waits for the block's other warps.
 // blockIdx.z takes every gridDim.z-th adapter of the rows.
-constexpr int SHRINK_WARPS = 8;
+template <int MT, int NJ> __host__ __device__ constexpr int shrink_stage() { return (16 * MT + 8 * NJ) * 128; }
 
-template <int MT, int NJ>
-__global__ void __launch_bounds__(SHRINK_WARPS * 32) shrink_mma_kernel(const bf16* __restrict__ x, int64_t stride, int cols, const bf16* __restrict__ f, int rank,
-                                                                       int r16, LoraRows rows, bf16* __restrict__ hx) {
-  extern __shared__ float part[];                      // [warps][16 MT][8 NJ]
+template <int MT, int NJ, int WARPS, int STAGES>
+__global__ void __launch_bounds__(WARPS * 32) shrink_mma_kernel(const bf16* __restrict__ x, int64_t stride, int cols, const bf16* __restrict__ f, int rank,
+                                                                int r16, LoraRows rows, bf16* __restrict__ hx) {
+  extern __shared__ __align__(128) uint8_t ring[];     // [warps][stages][rows of x, then factors][64]; then the warps' sums
   __shared__ int ids[16 * MT];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4, j0 = blockIdx.y * 8 * NJ;
   const int64_t t0 = (int64_t)blockIdx.x * 16 * MT;
   let_next_start();
   if (threadIdx.x < 16 * MT) ids[threadIdx.x] = t0 + threadIdx.x < rows.rows ? adapter_of(rows, t0 + threadIdx.x) : -1;
   __syncthreads();
-  constexpr int N = (16 * MT + 31) / 32;
-  Adapters<N> adapters(rows, t0, lane);
-  if (MT == 1) adapters.left[0] &= 0xffffu;            // half a warp's rows
-  const int blocks = (cols + 31) / 32;
+  constexpr int N = (16 * MT + 31) / 32, STAGE = shrink_stage<MT, NJ>();
+  Adapters<N> adapters;
+#pragma unroll
+  for (int i = 0; i < N; ++i) adapters.id[i] = 32 * i + lane < 16 * MT ? ids[32 * i + lane] : -1;
+  adapters.start();
+  const uint32_t mine = smem_u32(ring) + warp * STAGES * STAGE;
+  const int blocks = (cols + 63) / 64, n = blocks > warp ? (blocks - warp + WARPS - 1) / WARPS : 0;      // blocks of columns, and this warp's of them
+  float* part = reinterpret_cast<float*>(ring);        // [warps][16 MT][8 NJ]
   for (int d = 0;; ++d) {
     const int a = adapters.next();
     if (a < 0) break;
     if (d % gridDim.z != blockIdx.z) continue;
+    const bf16* fa = f + ((int64_t)a * rank + j0) * cols;
+    auto ask = [&](int i) {                            // this warp's i-th block of columns
+      if (i < n) {
+        const int c = (warp + i * WARPS) * 64 + lane % 8 * 8;
+        const uint32_t at = mine + i % STAGES * STAGE;
+#pragma unroll
+        for (int k = 0; k < (16 * MT + 8 * NJ) / 4; ++k) {
+          const int r = 4 * k + lane / 8;
+          const bool of_x = r < 16 * MT;
+          const bool in = c < cols && (of_x ? t0 + r < rows.rows : j0 + r - 16 * MT < rank);
+          const bf16* src = of_x ? x + (t0 + r) * stride + c : fa + (int64_t)(r - 16 * MT) * cols + c;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + r * 128 + ((lane % 8 ^ (r & 7)) << 4)), "l"(in ? src : x), "r"(in ? 16 : 0) : "memory");
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     float acc[MT][NJ][4];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -83,33 +106,34 @@ __global__ void __launch_bounds__(SHRINK_WARPS * 32) shrink_mma_kernel(const bf1
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
-    const bf16* fa = f + ((int64_t)a * rank + j0) * cols;
-#pragma unroll 2
-    for (int b = warp; b < blocks; b += SHRINK_WARPS) {
-      const int c = b * 32 + t * 8;
-      const bool in = c < cols;
-      uint4 fr[NJ], xa[MT][2];
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+    for (int i = 0; i < STAGES - 1; ++i) ask(i);
+    for (int i = 0; i < n; ++i) {
+      ask(i + STAGES - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+      __syncwarp();
+      const uint8_t* at = ring + (mine - smem_u32(ring)) + i % STAGES * STAGE;
+      auto piece = [&](int r, int c) { return reinterpret_cast<const bf16*>(at + r * 128 + ((c ^ (r & 7)) << 4)); };
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int64_t row = t0 + 16 * m + g + 8 * r;
-          xa[m][r] = in && row < rows.rows ? __ldg(reinterpret_cast<const uint4*>(x + row * stride + c)) : make_uint4(0, 0, 0, 0);
-        }
+      for (int k = 0; k < 4; ++k) {
+        uint32_t xf[MT][4];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        fr[j] = in && j0 + 8 * j + g < rank ? __ldg(reinterpret_cast<const uint4*>(fa + (int64_t)(8 * j + g) * cols + c)) : make_uint4(0, 0, 0, 0);
+        for (int m = 0; m < MT; ++m) ldsm4(xf[m], piece(16 * m + lane % 16, 2 * k + lane / 16));
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const uint32_t lo[4] = {xa[m][0].x, xa[m][1].x, xa[m][0].y, xa[m][1].y}, hi[4] = {xa[m][0].z, xa[m][1].z, xa[m][0].w, xa[m][1].w};
+        for (int j = 0; j < NJ; j += 2) {
+          uint32_t ff[4];
+          ldsm4(ff, piece(16 * MT + 8 * j + lane % 8 + lane / 16 * 8, 2 * k + lane / 8 % 2));
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          mma(acc[m][j], lo, fr[j].x, fr[j].y);
-          mma(acc[m][j], hi, fr[j].z, fr[j].w);
+          for (int m = 0; m < MT; ++m) {
+            mma(acc[m][j], xf[m], ff[0], ff[1]);
+            mma(acc[m][j + 1], xf[m], ff[2], ff[3]);
+          }
         }
       }
+      __syncwarp();                                    // read by all lanes: may be filled again
     }
-    __syncthreads();                                   // the sums of the adapter before have been read
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();                                   // the sums lie where the rings are
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -119,12 +143,12 @@ __global__ void __launch_bounds__(SHRINK_WARPS * 32) shrink_mma_kernel(const bf1
           *reinterpret_cast<float2*>(part + (warp * 16 * MT + 16 * m + g + 8 * r) * 8 * NJ + 8 * j + 2 * t) = make_float2(acc[m][j][2 * r], acc[m][j][2 * r + 1]);
     __syncthreads();
     const float scale = scaling_of(rows, a);
-    for (int e = threadIdx.x; e < 16 * MT * 8 * NJ; e += SHRINK_WARPS * 32) {
+    for (int e = threadIdx.x; e < 16 * MT * 8 * NJ; e += WARPS * 32) {
       const int row = e / (8 * NJ), j = e % (8 * NJ);
       if (ids[row] != a || j0 + j >= r16) continue;
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < SHRINK_WARPS; ++w) s += part[w * 16 * MT * 8 * NJ + e];
+      for (int w = 0; w < WARPS; ++w) s += part[w * 16 * MT * 8 * NJ + e];
       s *= scale;
       const bf16 high = __float2bfloat16_rn(s);
       const float rest = s - __bfloat162float(high);
@@ -132,46 +156,132 @@ __global__ void __launch_bounds__(SHRINK_WARPS * 32) shrink_mma_kernel(const bf1
       out[0] = high;
       out[r16] = __float2bfloat16_rn(isfinite(rest) ? rest : 0.f);
     }
+    __syncthreads();
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------------ product
-// Persistent, one CTA to an SM, tiles of 128 rows and BN columns, two accumulators.  Warp 0 fetches tiles of x and W by TMA into a ring of
-// stages, warps 2..5 fill the stages of the adapters' steps by hand, warp 1 issues the products, warps 6..9 drain one accumulator (tensor
-// memory, bias, bf16, shared memory, whole 128-byte lines) while the other one fills.  All of them walk the same list of steps, and
-// each finds a tile's adapters for itself from the rows' ids.
+// Persistent, tiles of 128 CTAS rows and BN columns, two accumulators.  With CTAS = 2 a pair of SMs works on one tile: each fetches its own
+// 128 rows of x and half of the columns of W, and the tensor cores of both read the other half from the neighbour.  That halves what has to come
+// from L2 for W, which is what bounds the product: with a 128 x 256 tile to one SM every 128 x 256 x 64 step fetched 48 KB, 12 TB/s over the
+// chip, and ran at 46 % of the tensor cores' rate (9216 rows 1024 -> 4096 without adapters: 89.9 us).
+//
+// Warp 0 fetches tiles of x and W by TMA into a ring of stages, warps 2..5 fill the stages of the adapters' steps by hand, warp 1 (of the
+// pair's first CTA) issues the products, warps 6..9 drain one accumulator (tensor memory, bias, bf16, shared memory, whole 128-byte lines)
+// while the other one fills.  All of them walk the same list of steps; warp 10 counts the adapters of the worker's tiles ahead of the others.
 //
 // 0 x NaN is NaN, so what an adapter holds must not meet other rows' zeros: numbers that are not finite are left out of the B tile, and the
-// rows of that adapter get their products from the slow loop at the end of the tile.
-constexpr int BM = 128, THREADS = 320;
+// rows of that adapter get their products from a loop at the end.
+constexpr int BM = 128, THREADS = 352, MOST_TILES = 512;   // MOST_TILES: of one worker in a launch
 constexpr uint32_t A_BYTES = BM * 128;
 constexpr uint64_t WAIT_NS = 1000ull * 1000ull * 1000ull;
-__host__ __device__ constexpr int stages_of(int bn) { return bn == 256 ? 4 : bn == 128 ? 6 : 8; }
-__host__ __device__ constexpr uint32_t ring_bytes(int bn) { return (uint32_t)stages_of(bn) * (A_BYTES + (uint32_t)bn * 128); }
-constexpr uint32_t OUT_BYTES = 4 * 32 * 128, BAR_BYTES = 512;
-__host__ __device__ constexpr uint32_t smem_of(int bn) { return ring_bytes(bn) + OUT_BYTES + BAR_BYTES + 1024; }
+__host__ __device__ constexpr uint32_t stage_bytes(int bn, int ctas) { return A_BYTES + (uint32_t)(bn / ctas) * 128; }
+__host__ __device__ constexpr int stages_of(int bn, int ctas) { return 192 * 1024 / (int)stage_bytes(bn, ctas); }
+__host__ __device__ constexpr uint32_t ring_bytes(int bn, int ctas) { return (uint32_t)stages_of(bn, ctas) * stage_bytes(bn, ctas); }
+constexpr uint32_t OUT_BYTES = 2 * 4 * 32 * 128, BAR_BYTES = 512 + 2 * MOST_TILES;
+__host__ __device__ constexpr uint32_t smem_of(int bn, int ctas) { return ring_bytes(bn, ctas) + OUT_BYTES + BAR_BYTES + 1024; }
 
+// The pair: addresses, barriers and tensor-core instructions that reach the neighbour.
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+// RELEASE: what this thread wrote goes first; that waits for all its stores to global memory too, some 1500 cycles where there are any.
+template <bool RELEASE>
+__device__ __forceinline__ void arrive_in_cluster(uint32_t bar) {
+  if (RELEASE) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  else asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ bool test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+// mbar_wait() that polls.
+__device__ __forceinline__ bool polling_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code, uint64_t limit_ns) {
+  for (int i = 0; i < 64; ++i)
+    if (test_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!*abort_flag) {
+    for (int i = 0; i < 64; ++i)
+      if (test_wait(bar, parity)) return true;
+    if (globaltimer_ns() - t0 > limit_ns) {
+      *abort_flag = 1;
+      if (*reinterpret_cast<volatile int*>(status) == 0) *reinterpret_cast<volatile int*>(status) = code;
+    }
+  }
+  return false;
+}
+template <int CTAS>
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1) : "memory");
+  if (CTAS == 2)                                       // may signal the neighbour's barrier
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+// For a converged warp: every lane computes the operands, so that they can stay in uniform registers, and one elected lane issues.
+template <int CTAS>
+__device__ __forceinline__ void mma_step(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  if (CTAS == 2)
+    asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accum) : "memory");
+  else
+    mma_ss_warp(d, a, b, idesc, accum);
+}
+// The barrier at this offset, in both CTAs of a pair, completes once the products so far have.
+template <int CTAS>
+__device__ __forceinline__ void commit_step(uint32_t bar) {
+  if (CTAS == 2)
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+                 "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar), "h"((uint16_t)3) : "memory");
+  else
+    tc_commit_warp(bar);
+}
+template <int CTAS>
+__device__ __forceinline__ void alloc_columns(uint32_t dst, uint32_t n) {
+  if (CTAS == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(n) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(dst, n);
+    tmem_relinquish();
+  }
+}
+template <int CTAS>
+__device__ __forceinline__ void free_columns(uint32_t tmem, uint32_t n) {
+  if (CTAS == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(n) : "memory");
+  else tmem_dealloc(tmem, n);
 }
 // W along its other axis: groups of 64 columns, each 64 rows of 128 bytes (rows run along the inner dimension).
 __device__ __forceinline__ uint64_t smem_desc_columns(uint32_t saddr) { return (smem_desc_sw128(saddr) & ~(0x3FFFull << 16)) | ((uint64_t)(8192 >> 4) << 16); }
 
-// Eight factors of one output column from j on; what is not finite is left out and reported.
+// Eight factors of one output column from j on.
 template <bool VEC>
-__device__ __forceinline__ uint4 factors8(const bf16* row, int j, int rank, uint32_t& bad) {
+__device__ __forceinline__ uint4 factors8(const bf16* row, int j, int rank) {
+  if (VEC) return j < rank ? __ldg(reinterpret_cast<const uint4*>(row + j)) : make_uint4(0, 0, 0, 0);
   uint32_t w[4];
-  if (VEC) {
-    const uint4 v = j < rank ? __ldg(reinterpret_cast<const uint4*>(row + j)) : make_uint4(0, 0, 0, 0);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = j + 2 * i < rank ? __bfloat16_as_ushort(row[j + 2 * i]) : 0, hi = j + 2 * i + 1 < rank ? __bfloat16_as_ushort(row[j + 2 * i + 1]) : 0;
-      w[i] = lo | hi << 16;
-    }
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = j + 2 * i < rank ? __bfloat16_as_ushort(row[j + 2 * i]) : 0, hi = j + 2 * i + 1 < rank ? __bfloat16_as_ushort(row[j + 2 * i + 1]) : 0;
+    w[i] = lo | hi << 16;
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// What is not finite becomes zero, and is reported.
+__device__ __forceinline__ uint4 finite8(uint4 v, uint32_t& bad) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t not_finite = __vcmpeq2(w[i] & 0x7f807f80u, 0x7f807f80u);
@@ -189,179 +299,247 @@ struct ProductParams {
   int32_t* status;
 };
 
-template <int BN, bool BACK, bool VEC>
-__global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const ProductParams p) {
-  constexpr int S = stages_of(BN);
-  constexpr uint32_t STAGE = A_BYTES + BN * 128;
+template <int BN, int CTAS, bool BACK, bool VEC>
+__global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_y,
+                    const ProductParams p) {
+  constexpr int S = stages_of(BN, CTAS), PART = BN / CTAS;        // PART: columns of W whose tile is in this CTA
+  constexpr uint32_t STAGE = stage_bytes(BN, CTAS);
   extern __shared__ uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
-  constexpr uint32_t BARS = ring_bytes(BN) + OUT_BYTES;
-  // full[s], empty[s], granted[s], then for both accumulators: filled, drained, and the loaders' report
+  constexpr uint32_t BARS = ring_bytes(BN, CTAS) + OUT_BYTES;
+  // full[s] (the first CTA's counts for both), empty[s], granted[s], then for both accumulators: filled, drained
   auto bar = [&](int i) { return base + BARS + 8u * (uint32_t)i; };
-  constexpr int EMPTY = S, GRANTED = 2 * S, FILLED = 3 * S, DRAINED = 3 * S + 2, REPORT = 3 * S + 4;
+  constexpr int EMPTY = S, GRANTED = 2 * S, FILLED = 3 * S, DRAINED = 3 * S + 2;
+  static_assert(8 * (3 * S + 4) <= 256, "barriers");
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + BARS + 256);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + BARS + 260);
-  volatile uint32_t* reports = reinterpret_cast<volatile uint32_t*>(gbase + BARS + 264);        // [2][4]
-  auto wait = [&](int i, int phase) { return mbar_wait(bar(i), (uint32_t)(phase & 1), abort_flag, p.status, 200 + i, WAIT_NS); };
-
+  volatile int* counted = reinterpret_cast<volatile int*>(gbase + BARS + 268);                 // tiles whose adapters have been counted
+  volatile uint16_t* counts = reinterpret_cast<volatile uint16_t*>(gbase + BARS + 512);
+  volatile uint32_t* bad_factors = reinterpret_cast<volatile uint32_t*>(gbase + BARS + 264);
+  auto wait = [&](int i, int phase) { return (CTAS == 2 ? polling_wait : mbar_wait)(bar(i), (uint32_t)(phase & 1), abort_flag, p.status, 200 + i, WAIT_NS); };
+  const uint32_t rank = CTAS == 2 ? cta_rank() : 0;
+  auto first_cta = [&](uint32_t addr) { return CTAS == 2 ? in_cta(addr, 0) : addr; };
   if (tid == 0) {
     *abort_flag = 0;
-    for (int i = 0; i < 3 * S; ++i) mbar_init(bar(i), 1u);
-    for (int i = 0; i < 2; ++i) { mbar_init(bar(FILLED + i), 1u); mbar_init(bar(DRAINED + i), 4u); mbar_init(bar(REPORT + i), 4u); }
+    *bad_factors = 0;
+    *counted = 0;
+    for (int i = 0; i < 3 * S; ++i) mbar_init(bar(i), i < S ? CTAS : 1u);
+    for (int i = 0; i < 2; ++i) { mbar_init(bar(FILLED + i), 1u); mbar_init(bar(DRAINED + i), 4u * CTAS); }
     fence_mbar_init();
     prefetch_tmap(&tm_x);
     prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_y);
   }
-  if (warp == 1) {
-    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 2 * BN);
-    tmem_relinquish();
-  }
+  if (warp == 1) alloc_columns<CTAS>(smem_u32(const_cast<uint32_t*>(tmem_slot)), 2 * BN);
+  __syncwarp();
   tc_fence_before();
-  __syncthreads();
+  if (CTAS == 2) cluster_sync();
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int n_tiles = (p.N + BN - 1) / BN, tiles = (int)((p.rows.rows + BM - 1) / BM) * n_tiles;
-  const int nk = (p.K + 63) / 64, inner = 2 * p.r16, chunks = (inner + 63) / 64;
-  int step = 0, it = 0;
+  const int n_tiles = (p.N + BN - 1) / BN, tiles = (int)((p.rows.rows + BM * CTAS - 1) / (BM * CTAS)) * n_tiles;
+  const int workers = gridDim.x / CTAS, worker = blockIdx.x / CTAS;
+  const int nk = (p.K + 63) / 64, inner = 2 * p.r16;      // inner: columns of an adapter; a tile's adapters lie one behind the other
+  int it = 0;
+  using Tile = Adapters<4 * CTAS>;
+  auto count_of = [&](int i) {                         // of this worker's i-th tile
+    if (*counted <= i) {
+      const uint64_t t0 = globaltimer_ns();
+      while (*counted <= i && !*abort_flag)
+        if (globaltimer_ns() - t0 > WAIT_NS) {
+          *abort_flag = 1;
+          if (*reinterpret_cast<volatile int*>(p.status) == 0) *reinterpret_cast<volatile int*>(p.status) = 299;
+        }
+    }
+    __threadfence_block();
+    return (int)counts[i];
+  };
+  auto tile_row = [&](int tile) { return (int64_t)(tile / n_tiles) * BM * CTAS; };
+
+  // Stages go round; `odd` is the parity of the round.  A fresh barrier counts as having completed the phase before its first.
+  int s = 0, odd = 0;
+  auto advance = [&] { if (++s == S) { s = 0; odd ^= 1; } };
 
   if (warp == 0) {
     // ---- tiles of x and W
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-      const int m0 = tile / n_tiles * BM, n0 = tile % n_tiles * BN;
-      const int more = Adapters<4>(p.rows, m0, lane).count() * chunks;
+    for (int tile = worker; tile < tiles; tile += workers, ++it) {
+      const int m0 = (int)tile_row(tile) + rank * BM, n0 = tile % n_tiles * BN + rank * PART;
+      // Lane 0 alone waits for stages, in the order of the steps, and grants those of the adapters' steps to the warps that fill them: a
+      // barrier tells two neighbouring phases apart and no more, so nobody may wait for one that others can go past.
       if (lane == 0) {
-        for (int k = 0; k < nk + more; ++k) {
-          const int s = (step + k) % S, round = (step + k) / S;
-          // This lane alone waits for stages, in the order of the steps, and grants those of the adapters' steps to the warps that fill them: a
-          // barrier tells two neighbouring phases apart and no more, so nobody may wait for one that others can go past.
-          if (round > 0) wait(EMPTY + s, round - 1);
-          if (k >= nk) mbar_arrive(bar(GRANTED + s));
-          if (k >= nk || *abort_flag) continue;
-          const uint32_t a = base + s * STAGE, b = a + A_BYTES;
-          mbar_expect_tx(bar(s), STAGE);
-          tma_load_2d(a, &tm_x, bar(s), k * 64, m0);
+        bool go = true;
+        for (int k = 0; k < nk; ++k, advance()) {
+          go = wait(EMPTY + s, odd ^ 1) && go;
+          if (!go) continue;
+          const uint32_t a = base + s * STAGE, b = a + A_BYTES, full = first_cta(bar(s));
+          if (rank == 0) mbar_expect_tx(bar(s), STAGE * CTAS);
+          if (CTAS == 2 && rank == 0) mbar_arrive(bar(s));          // for the neighbour, whose bytes are counted here: an arrival from there would cost it a fence
+          tma_load_2d<CTAS>(a, &tm_x, full, k * 64, m0);
           if (!BACK) {
-            tma_load_2d(b, &tm_w, bar(s), k * 64, n0);
+            tma_load_2d<CTAS>(b, &tm_w, full, k * 64, n0);
           } else {
 #pragma unroll
-            for (int c = 0; c < BN / 64; ++c) tma_load_2d(b + c * 8192, &tm_w, bar(s), n0 + c * 64, k * 64);
+            for (int c = 0; c < PART / 64; ++c) tma_load_2d<CTAS>(b + c * 8192, &tm_w, full, n0 + c * 64, k * 64);
           }
         }
-      }
-      step += nk + more;
-      __syncwarp();
-    }
-  } else if (warp == 1) {
-    // ---- products
-    constexpr uint32_t ID = make_idesc_bf16(BM, BN, BACK), ID_ADAPTERS = make_idesc_bf16(BM, BN, 0);
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++it) {
-      const int m0 = tile / n_tiles * BM;
-      const int more = Adapters<4>(p.rows, m0, lane).count() * chunks;
-      const uint32_t acc = tmem + (it & 1) * BN;
-      if (lane == 0) {
-        if (it >= 2) wait(DRAINED + (it & 1), it / 2 - 1);
-        tc_fence_after();
-        for (int k = 0; k < nk + more; ++k) {
-          const int s = (step + k) % S;
-          wait(s, (step + k) / S);
-          tc_fence_after();
-          const uint32_t a = base + s * STAGE, b = a + A_BYTES;
-          const uint64_t da = smem_desc_sw128(a), db = BACK && k < nk ? smem_desc_columns(b) : smem_desc_sw128(b);
-          const int left = inner - (k - nk) % chunks * 64, k16 = k < nk || left >= 64 ? 4 : left / 16;
-          const uint64_t along = BACK && k < nk ? 128 : 2;
-          for (int i = 0; i < k16; ++i) mma_ss(acc, da + 2 * i, db + along * i, k < nk ? ID : ID_ADAPTERS, k > 0 || i > 0 ? 1u : 0u);
-          tc_commit(bar(EMPTY + s));
+        const int more = (count_of(it) * inner + 63) / 64;
+        for (int k = 0; k < more; ++k, advance()) {
+          wait(EMPTY + s, odd ^ 1);
+          mbar_arrive(bar(GRANTED + s));
         }
-        tc_commit(bar(FILLED + (it & 1)));
       }
-      step += nk + more;
       __syncwarp();
     }
-  } else if (warp < 6) {
+  } else if (warp == 1 && rank == 0) {
+    // ---- products
+    constexpr uint32_t ID = make_idesc_bf16(BM * CTAS, BN, BACK), ID_ADAPTERS = make_idesc_bf16(BM * CTAS, BN, 0);
+    const uint64_t a0 = smem_desc_sw128(base), b0 = smem_desc_sw128(base + A_BYTES), w0 = BACK ? smem_desc_columns(base + A_BYTES) : b0;
+    constexpr uint64_t ALONG = BACK ? 128 : 2;         // 16 more of the inner dimension
+    for (int tile = worker; tile < tiles; tile += workers, ++it) {
+      const uint32_t acc = tmem + (it & 1) * BN;
+      if (it >= 2) wait(DRAINED + (it & 1), it / 2 - 1);
+      tc_fence_after();
+      for (int k = 0; k < nk; ++k, advance()) {
+        wait(s, odd);
+        tc_fence_after();
+        const uint64_t a = a0 + (uint32_t)s * (STAGE >> 4), b = w0 + (uint32_t)s * (STAGE >> 4);
+        mma_step<CTAS>(acc, a, b, ID, k > 0 ? 1u : 0u);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) mma_step<CTAS>(acc, a + 2 * i, b + ALONG * i, ID, 1u);
+        commit_step<CTAS>(bar(EMPTY + s));
+      }
+      for (int left = count_of(it) * inner; left > 0; left -= 64, advance()) {
+        wait(s, odd);
+        tc_fence_after();
+        const uint64_t a = a0 + (uint32_t)s * (STAGE >> 4), b = b0 + (uint32_t)s * (STAGE >> 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * i < left) mma_step<CTAS>(acc, a + 2 * i, b + 2 * i, ID_ADAPTERS, 1u);
+        commit_step<CTAS>(bar(EMPTY + s));
+      }
+      commit_step<CTAS>(bar(FILLED + (it & 1)));
+    }
+  } else if (warp >= 2 && warp < 6) {
     // ---- the adapters' steps: h as the A tile, with zeros in the rows of other adapters, and B_a as the B tile
     const int w = warp - 2, me = w * 32 + lane;
     uint32_t grants = 0;                               // of each stage: the phase to wait for
+    Tile adapters;
     wait_for_stream();                                 // hx is made by the kernel in front
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++it) {
-      const int m0 = tile / n_tiles * BM, n0 = tile % n_tiles * BN;
-      Adapters<4> adapters(p.rows, m0, lane);
-      const int mine = w == 0 ? adapters.id[0] : w == 1 ? adapters.id[1] : w == 2 ? adapters.id[2] : adapters.id[3];
-      step += nk;
+    for (int tile = worker; tile < tiles; tile += workers, ++it) {
+      const int64_t row0 = tile_row(tile);
+      const int n0 = tile % n_tiles * BN + rank * PART;
+      adapters.load(p.rows, row0, lane);
+      adapters.start();
+      int mine = -1;                                   // of row `me` of this CTA's rows
+#pragma unroll
+      for (int i = 0; i < 4 * CTAS; ++i)
+        if (i == (int)rank * 4 + w) mine = adapters.id[i];
+      s = (s + nk) % S;
       uint32_t bad = 0;
-      for (int a = adapters.next(); a >= 0; a = adapters.next()) {
-        for (int c = 0; c < chunks; ++c, ++step) {
-          const int pieces = min(8, (inner - c * 64) / 8);
-          const uint4* h = reinterpret_cast<const uint4*>(p.hx + (int64_t)(m0 + me) * inner + c * 64);
-          uint4 av[8];
+      const uint4* h = reinterpret_cast<const uint4*>(p.hx + (row0 + rank * BM + me) * inner);
+      const int left = count_of(it) * inner / 8;       // pieces of eight columns
+      int a = -1, q = 0;                               // the adapter, and the column of it, that the next piece is
+      for (int first = 0; first < left; first += 8, advance()) {
+        const int pieces = min(8, left - first);
+        constexpr int BR = (PART + 127) / 128;
+        uint4 av[8], bv[BR][8];                        // both tiles are on their way before the stage is free
 #pragma unroll
-          for (int i = 0; i < 8; ++i) av[i] = i < pieces && mine == a ? *(h + i) : make_uint4(0, 0, 0, 0);
-          const int s = step % S;
-          if (lane == 0) wait(GRANTED + s, (int)(grants >> s));
-          __syncwarp();
-          grants ^= 1u << s;
-          const uint32_t at = base + s * STAGE;
-          for (int r = me; r < BN; r += 128) {
-            const bool real = n0 + r < p.N;
-            const bf16* row = p.f + ((int64_t)a * p.N + (real ? n0 + r : 0)) * p.rank;
+        for (int i = 0; i < 8; ++i) {
+          const bool in = i < pieces;
+          if (in && q == 0) a = adapters.next();
+          av[i] = in && mine == a ? h[q / 8] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if (i >= pieces) break;
-              const int q = c * 64 + 8 * i, j = q >= p.r16 ? q - p.r16 : q;
-              const uint4 v = factors8<VEC>(row, j, real ? p.rank : 0, bad);
-              sts_128(at + A_BYTES + r * 128 + ((i ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
-            }
+          for (int r = 0; r < BR; ++r) {
+            const bool real = in && me + 128 * r < PART && n0 + me + 128 * r < p.N;
+            bv[r][i] = real ? factors8<VEC>(p.f + ((int64_t)a * p.N + n0 + me + 128 * r) * p.rank, q >= p.r16 ? q - p.r16 : q, p.rank) : make_uint4(0, 0, 0, 0);
           }
+          if (in) q = q + 8 == inner ? 0 : q + 8;
+        }
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < pieces) sts_128(at + me * 128 + ((i ^ (me & 7)) << 4), av[i].x, av[i].y, av[i].z, av[i].w);
-          fence_proxy_async_smem();
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          if (me == 0) mbar_arrive(bar(s));
+        for (int r = 0; r < BR; ++r)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) bv[r][i] = finite8(bv[r][i], bad);
+        if (lane == 0) wait(GRANTED + s, (int)(grants >> s));
+        __syncwarp();
+        grants ^= 1u << s;
+        const uint32_t at = base + s * STAGE;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i >= pieces) break;
+          sts_128(at + me * 128 + ((i ^ (me & 7)) << 4), av[i].x, av[i].y, av[i].z, av[i].w);
+#pragma unroll
+          for (int r = 0; r < BR; ++r) {
+            const uint4& v = bv[r][i];
+            if (PART >= 128 || me < PART) sts_128(at + A_BYTES + (me + 128 * r) * 128 + ((i ^ (me & 7)) << 4), v.x, v.y, v.z, v.w);
+          }
+        }
+        fence_proxy_async_smem();
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (me == 0) {
+          if (CTAS == 2) arrive_in_cluster<true>(in_cta(bar(s), 0));
+          else mbar_arrive(bar(s));
         }
       }
-      bad = __any_sync(0xffffffffu, bad != 0);
-      if (lane == 0) {
-        if (it >= 2) wait(DRAINED + (it & 1), it / 2 - 1);
-        reports[(it & 1) * 4 + w] = bad;
-        mbar_arrive(bar(REPORT + (it & 1)));
+      if (bad) {                                       // for the loop at the end, in both CTAs
+        const uint32_t at = smem_u32(const_cast<uint32_t*>(bad_factors));
+        if (CTAS == 1) *bad_factors = 1;
+        else
+          for (int r = 0; r < CTAS; ++r) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_cta(at, r)), "r"(1u) : "memory");
       }
       __syncwarp();
     }
-  } else {
-    // ---- results: warp w may read tensor-memory lanes 32 (w % 4) ..., a row to a thread
+  } else if (warp == 10) {
+    // ---- how many adapters each tile has
+    for (int tile = worker; tile < tiles; tile += workers, ++it) {
+      Tile adapters;
+      adapters.load(p.rows, tile_row(tile), lane);
+      const int n = adapters.count();
+      if (lane == 0) {
+        counts[it] = (uint16_t)n;
+        __threadfence_block();
+        *counted = it + 1;
+      }
+    }
+  } else if (warp >= 6) {
+    // ---- results: warp w may read tensor-memory lanes 32 (w % 4) ..., a row to a thread; 32 rows and 64 columns at a time go out by TMA from one
+    // of two buffers
     const int q = warp & 3;
-    const uint32_t out = base + ring_bytes(BN) + q * 4096;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++it) {
-      const int64_t m0 = (int64_t)(tile / n_tiles) * BM + q * 32;
-      const int n0 = tile % n_tiles * BN;
-      wait(REPORT + (it & 1), it / 2);                 // read before DRAINED, which lets the loaders write the next one here
-      const volatile uint32_t* r = reports + (it & 1) * 4;
-      const bool bad = r[0] | r[1] | r[2] | r[3];
+    int turn = 0;
+    for (int tile = worker; tile < tiles; tile += workers, ++it) {
+      const int m0 = (int)tile_row(tile) + rank * BM + q * 32, n0 = tile % n_tiles * BN;
       wait(FILLED + (it & 1), it / 2);
       tc_fence_after();
       const uint32_t acc = tmem + (it & 1) * BN + ((uint32_t)(q * 32) << 16);
 #pragma unroll 1
-      for (int c = 0; c < BN / 64; ++c) {
+      for (int c = 0; c < BN / 64; ++c, turn ^= 1) {
+        const int n = n0 + c * 64;
         uint32_t v[64];
         tmem_ld32(acc + c * 64, v);
         tmem_ld32(acc + c * 64 + 32, v + 32);
+        uint4 b[8];
+        if (p.bias) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) b[i] = n + 8 * i < p.N ? __ldg(reinterpret_cast<const uint4*>(p.bias + n) + i) : make_uint4(0, 0, 0, 0);
+        }
+        const uint32_t out = base + ring_bytes(BN, CTAS) + (q * 2 + turn) * 4096;
+        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");           // the store from this buffer has read it
         tmem_ld_wait32(v);
         tmem_ld_wait32(v + 32);
+        __syncwarp();
         if (c == BN / 64 - 1) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(DRAINED + (it & 1)));
+          if (lane == 0) {
+            if (CTAS == 1) mbar_arrive(bar(DRAINED + (it & 1)));
+            else arrive_in_cluster<false>(in_cta(bar(DRAINED + (it & 1)), 0));   // the first CTA issues the products
+          }
         }
-        const int n = n0 + c * 64;
-        if (n >= p.N) continue;
         if (p.bias) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            if (n + 8 * i >= p.N) break;
-            const uint4 b = __ldg(reinterpret_cast<const uint4*>(p.bias + n) + i);
-            const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
+            const uint32_t bw[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               v[8 * i + 2 * e] = __float_as_uint(__uint_as_float(v[8 * i + 2 * e]) + __uint_as_float(bw[e] << 16));
@@ -369,7 +547,6 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
             }
           }
         }
-        __syncwarp();
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           uint32_t o[4];
@@ -377,41 +554,47 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
           for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(__uint_as_float(v[8 * i + 2 * e]), __uint_as_float(v[8 * i + 2 * e + 1]));
           sts_128(out + lane * 128 + ((i ^ (lane & 7)) << 4), o[0], o[1], o[2], o[3]);
         }
+        fence_proxy_async_smem();
         __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int row = i * 4 + lane / 8, piece = lane % 8;
-          const uint4 o = lds_128(out + row * 128 + ((piece ^ (row & 7)) << 4));
-          if (m0 + row < p.rows.rows && n + 8 * piece < p.N) *reinterpret_cast<uint4*>(p.y + (m0 + row) * p.N + n + 8 * piece) = o;
+        if (lane == 0) {                               // rows and columns behind the last are left out by the copy
+          if (m0 < p.rows.rows && n < p.N && !*abort_flag)
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+                         ::"l"(reinterpret_cast<uint64_t>(&tm_y)), "r"(out), "r"(n), "r"(m0) : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
       }
-      if (bad && !*abort_flag) {
-        __syncwarp();
-        const int64_t t = m0 + lane;
-        const int a = t < p.rows.rows ? adapter_of(p.rows, t) : -1;
-        if (a >= 0)
-          for (int n = n0; n < min(n0 + BN, p.N); ++n) {
-            float s = 0.f;
-            bool any = false;
-            for (int j = 0; j < p.rank; ++j) {
-              const float v = __bfloat162float(p.f[((int64_t)a * p.N + n) * p.rank + j]);
-              if (isfinite(v)) continue;
-              any = true;
-              s += (__bfloat162float(p.hx[t * inner + j]) + __bfloat162float(p.hx[t * inner + p.r16 + j])) * v;
-            }
-            if (any) p.y[t * p.N + n] = __float2bfloat16_rn(__bfloat162float(p.y[t * p.N + n]) + s);
-          }
-      }
     }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   if (*abort_flag) {                                   // copies that may still be in flight get time to land
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
   }
+  __syncwarp();
   tc_fence_before();
-  __syncthreads();
+  if (CTAS == 2) cluster_sync();                       // nobody leaves while the neighbour may still read or signal here
+  else __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, 2 * BN);
+  if (warp == 1) free_columns<CTAS>(tmem, 2 * BN);
+  if (!*bad_factors || *abort_flag) return;
+  // Some factor is not finite: this CTA's tiles once more, for what was left out of them.
+  for (int tile = worker; tile < tiles; tile += workers) {
+    const int n0 = tile % n_tiles * BN;
+    for (int e = tid; e < BM * BN; e += THREADS) {
+      const int64_t t = tile_row(tile) + rank * BM + e / BN;
+      const int n = n0 + e % BN, a = t < p.rows.rows ? adapter_of(p.rows, t) : -1;
+      if (a < 0 || n >= p.N) continue;
+      float sum = 0.f;
+      bool any = false;
+      for (int j = 0; j < p.rank; ++j) {
+        const float v = __bfloat162float(p.f[((int64_t)a * p.N + n) * p.rank + j]);
+        if (isfinite(v)) continue;
+        any = true;
+        sum += (__bfloat162float(p.hx[t * inner + j]) + __bfloat162float(p.hx[t * inner + p.r16 + j])) * v;
+      }
+      if (any) p.y[t * p.N + n] = __float2bfloat16_rn(__bfloat162float(p.y[t * p.N + n]) + sum);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------------- gather
@@ -534,35 +717,44 @@ __global__ void __launch_bounds__(256) turn_kernel(const bf16* __restrict__ in, 
 LoraRows rows_of(const Lora& l) { return LoraRows{l.ids, l.id_bytes, l.rows_per_id, l.rows, l.n, l.scaling, l.scaling_value}; }
 int r16_of(const Lora& l) { return (l.rank + 15) / 16 * 16; }
 
-template <int MT, int NJ>
+template <int MT, int NJ, int WARPS, int STAGES>
 int launch_shrink(const Lora& l, const bf16* x, int64_t stride, int cols, const bf16* f, bf16* hx, int sms, cudaStream_t s) {
-  constexpr int smem = SHRINK_WARPS * 16 * MT * 8 * NJ * 4;
-  if (smem > 48 * 1024)
-    if (const int rc = opt_in_smem(reinterpret_cast<const void*>(shrink_mma_kernel<MT, NJ>), smem)) return rc;
+  constexpr int smem = WARPS * STAGES * shrink_stage<MT, NJ>();
+  static_assert(WARPS * 16 * MT * 8 * NJ * 4 <= smem, "the warps' sums");
+  auto kernel = shrink_mma_kernel<MT, NJ, WARPS, STAGES>;
+  if (const int rc = opt_in_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
   const int64_t tiles = (l.rows + 16 * MT - 1) / (16 * MT);
   const int js = (r16_of(l) + 8 * NJ - 1) / (8 * NJ);
   // where there are SMs to spare, a tile's adapters are shared out too
   const int z = (int)std::max<int64_t>(1, std::min<int64_t>({l.n, 16 * MT, l.rows, 2 * sms / std::max<int64_t>(1, tiles * js)}));
-  shrink_mma_kernel<MT, NJ><<<dim3((unsigned)tiles, js, z), SHRINK_WARPS * 32, smem, s>>>(x, stride, cols, f, l.rank, r16_of(l), rows_of(l), hx);
+  kernel<<<dim3((unsigned)tiles, js, z), WARPS * 32, smem, s>>>(x, stride, cols, f, l.rank, r16_of(l), rows_of(l), hx);
   return cuda_fail(cudaGetLastError(), "lora shrink launch");
 }
 
-template <int BN, bool BACK>
-int launch_product(const CUtensorMap& tx, const CUtensorMap& tw, const ProductParams& p, int sms, cudaStream_t s) {
+template <int BN, int CTAS, bool BACK>
+int launch_product(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& ty, const ProductParams& p, int sms, cudaStream_t s) {
   const bool vec = p.rank % 8 == 0 && (reinterpret_cast<uintptr_t>(p.f) & 15) == 0;
-  auto kernel = vec ? lora_product_kernel<BN, BACK, true> : lora_product_kernel<BN, BACK, false>;
-  if (const int rc = opt_in_smem(reinterpret_cast<const void*>(kernel), (int)smem_of(BN))) return rc;
-  const int64_t tiles = (p.rows.rows + BM - 1) / BM * ((p.N + BN - 1) / BN);
-  return cuda_fail(launch_early(kernel, dim3((unsigned)std::min<int64_t>(tiles, sms)), THREADS, smem_of(BN), s, tx, tw, p), "lora product launch");
+  auto kernel = vec ? lora_product_kernel<BN, CTAS, BACK, true> : lora_product_kernel<BN, CTAS, BACK, false>;
+  if (const int rc = opt_in_smem(reinterpret_cast<const void*>(kernel), (int)smem_of(BN, CTAS))) return rc;
+  const int64_t tiles = (p.rows.rows + BM * CTAS - 1) / (BM * CTAS) * ((p.N + BN - 1) / BN);
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {CTAS, 1, 1};
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(tiles, sms / CTAS) * CTAS); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem_of(BN, CTAS); cfg.stream = s;
+  cfg.attrs = attr; cfg.numAttrs = CTAS == 2 ? 2 : 1;
+  return cuda_fail(cudaLaunchKernelEx(&cfg, kernel, tx, tw, ty, p), "lora product launch");
 }
 
-// The width of the tiles: the one whose waves of tiles take least, 256 columns counting 256, 128 of them 136 (twice the steps for the same
-// products) and 64 of them 96 (their operands come from shared memory slower than they are multiplied).
-int columns_of(int64_t rows, int N, int sms) {
-  const int64_t m = (rows + BM - 1) / BM;
-  auto cost = [&](int bn, int each) { return (m * ((N + bn - 1) / bn) + sms - 1) / sms * each; };
-  const int64_t c256 = cost(256, 256), c128 = cost(128, 136), c64 = cost(64, 96);
-  return c256 <= c128 && c256 <= c64 ? 256 : c128 <= c64 ? 128 : 64;
+// Columns of a tile, and whether a pair of SMs shares it: the form whose waves of tiles take least, in the time of a step.  A pair's
+// 256 x 256 tile counts 256; 128 x 128 to one SM, which waits for L2, 224; 128 x 64 176.
+struct Shape { int columns, ctas; };
+Shape shape_of(int64_t rows, int N, int sms) {
+  auto waves = [&](int m, int n, int workers) { return ((rows + m - 1) / m * ((N + n - 1) / n) + workers - 1) / workers; };
+  const int64_t pair = waves(256, 256, sms / 2) * 256, wide = waves(128, 128, sms) * 224, narrow = waves(128, 64, sms) * 176;
+  return pair <= wide && pair <= narrow ? Shape{256, 2} : wide <= narrow ? Shape{128, 1} : Shape{64, 1};
 }
 
 }  // namespace
@@ -574,7 +766,13 @@ extern "C" {
 
 // bf16 whose rows TMA can address; the host sees to it that the tensors are aligned.
 int tdb_lora_umma_applies(const Lora* l) {
-  return l->dtype == TDB_DTYPE_BF16 && l->cols % 8 == 0 && l->features % 8 == 0 && l->rows < (int64_t)1 << 30;
+  int sms = 0;
+  if (l->dtype != TDB_DTYPE_BF16 || l->cols % 8 || l->features % 8 || l->rows >= (int64_t)1 << 30 || device_sms(&sms)) return 0;
+  for (const int N : {l->features, l->cols}) {
+    const Shape s = shape_of(l->rows, N, sms);
+    if ((l->rows + BM * s.ctas - 1) / (BM * s.ctas) * ((N + s.columns - 1) / s.columns) > (int64_t)MOST_TILES * (sms / s.ctas)) return 0;     // outputs of some 5 GB
+  }
+  return 1;
 }
 
 int64_t tdb_lora_inner(const Lora* l) { return 2 * r16_of(*l); }
@@ -586,10 +784,10 @@ int tdb_lora_umma_shrink(const Lora* l, int back, const void* f, void* hx, void*
   const int64_t stride = back ? l->dy_stride : l->x_stride;
   const int cols = back ? l->features : l->cols;
   auto run = [&](auto launch) { return launch(*l, x, stride, cols, (const bf16*)f, (bf16*)hx, sms, (cudaStream_t)stream); };
-  const int mt = l->rows <= 16 * sms ? 1 : l->rows <= 64 * sms ? 2 : 4;
-  if (l->rank <= 16) return run(mt == 1 ? launch_shrink<1, 2> : mt == 2 ? launch_shrink<2, 2> : launch_shrink<4, 2>);
-  if (l->rank <= 32) return run(mt == 1 ? launch_shrink<1, 4> : mt == 2 ? launch_shrink<2, 4> : launch_shrink<4, 4>);
-  return run(mt == 1 ? launch_shrink<1, 8> : launch_shrink<2, 8>);
+  const bool few = l->rows <= 16 * sms;
+  if (l->rank <= 16) return run(few ? launch_shrink<1, 2, 8, 2> : launch_shrink<2, 2, 4, 4>);
+  if (l->rank <= 32) return run(few ? launch_shrink<1, 4, 8, 2> : launch_shrink<2, 4, 4, 3>);
+  return run(few ? launch_shrink<1, 8, 8, 2> : launch_shrink<2, 8, 4, 2>);
 }
 
 int tdb_lora_umma_product(const Lora* l, int back, const void* f, const void* hx, void* y, int32_t* status, void* stream) {
@@ -597,13 +795,15 @@ int tdb_lora_umma_product(const Lora* l, int back, const void* f, const void* hx
   if ((rc = device_sms(&sms))) return rc;
   const int K = back ? l->features : l->cols, N = back ? l->cols : l->features;
   const ProductParams p{rows_of(*l), (const bf16*)hx, (const bf16*)f, back ? nullptr : (const bf16*)l->bias, K, N, l->rank, r16_of(*l), (bf16*)y, status};
-  const int bn = columns_of(l->rows, N, sms);
-  CUtensorMap tx, tw;
+  const Shape shape = shape_of(l->rows, N, sms);
+  CUtensorMap tx, tw, ty;
   if ((rc = bf16_map_2d(&tx, back ? l->dy : l->x, K, l->rows, back ? l->dy_stride : l->x_stride, BM, back ? "dy" : "x"))) return rc;
-  if ((rc = bf16_map_2d(&tw, l->w, l->cols, l->features, l->cols, back ? 64 : bn, "weight"))) return rc;
+  if ((rc = bf16_map_2d(&tw, l->w, l->cols, l->features, l->cols, back ? 64 : shape.columns / shape.ctas, "weight"))) return rc;
+  if ((rc = bf16_map_2d(&ty, y, N, l->rows, N, 32, "y"))) return rc;
   cudaStream_t s = (cudaStream_t)stream;
-  if (back) return bn == 256 ? launch_product<256, true>(tx, tw, p, sms, s) : bn == 128 ? launch_product<128, true>(tx, tw, p, sms, s) : launch_product<64, true>(tx, tw, p, sms, s);
-  return bn == 256 ? launch_product<256, false>(tx, tw, p, sms, s) : bn == 128 ? launch_product<128, false>(tx, tw, p, sms, s) : launch_product<64, false>(tx, tw, p, sms, s);
+  auto run = [&](auto launch) { return launch(tx, tw, ty, p, sms, s); };
+  if (back) return run(shape.columns == 256 ? launch_product<256, 2, true> : shape.columns == 128 ? launch_product<128, 1, true> : launch_product<64, 1, true>);
+  return run(shape.columns == 256 ? launch_product<256, 2, false> : shape.columns == 128 ? launch_product<128, 1, false> : launch_product<64, 1, false>);
 }
 
 int tdb_lora_turn(const void* in, int n, int rows, int cols, void* out, void* stream) {
