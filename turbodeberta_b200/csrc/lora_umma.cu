@@ -21,18 +21,36 @@ namespace {
 using bf16 = __nv_bfloat16;
 
 // Goes through the adapters of 32 N rows, each once, in the order of their first rows; a whole warp holds the ids, lane l those of
-// rows l, l + 32, ...  load() only asks for them, so that their way from memory can pass beside other work.
+// rows l, l + 32, ...
 template <int N>
 struct Adapters {
-  int id[N];
+  int id[N], high[N];
   uint32_t left[N];
-  __device__ __forceinline__ void load(const LoraRows& rows, int64_t t0, int lane) {
+  // ask() only starts the loads, so that their way from memory can pass beside other work; start() is the first to look at them.
+  __device__ __forceinline__ void ask(const LoraRows& rows, int64_t t0, int lane) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) id[i] = t0 + 32 * i + lane < rows.rows ? adapter_of(rows, t0 + 32 * i + lane) : -1;
+    for (int i = 0; i < N; ++i) {
+      id[i] = high[i] = -1;
+      const int64_t row = t0 + 32 * i + lane;
+      if (row >= rows.rows) continue;
+      const int64_t at = rows.rows_per_id == 1 ? row : row / rows.rows_per_id;
+      if (!rows.ids) {
+        id[i] = high[i] = 0;
+      } else if (rows.id_bytes == 8) {
+        const int2 v = static_cast<const int2*>(rows.ids)[at];
+        id[i] = v.x; high[i] = v.y;
+      } else {
+        id[i] = static_cast<const int*>(rows.ids)[at];
+        high[i] = 0;
+      }
+    }
   }
-  __device__ __forceinline__ void start() {
+  __device__ __forceinline__ void start(int n) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) left[i] = __ballot_sync(0xffffffffu, id[i] >= 0);
+    for (int i = 0; i < N; ++i) {
+      id[i] = high[i] == 0 && id[i] >= 0 && id[i] < n ? id[i] : -1;
+      left[i] = __ballot_sync(0xffffffffu, id[i] >= 0);
+    }
   }
   // The next adapter, or -1.
   __device__ __forceinline__ int next() {
@@ -46,8 +64,7 @@ struct Adapters {
     }
     return a;
   }
-  __device__ __forceinline__ int count() {
-    start();
+  __device__ __forceinline__ int count() {              // goes through them
     int n = 0;
     while (next() >= 0) ++n;
     return n;
@@ -74,8 +91,8 @@ __global__ void __launch_bounds__(WARPS * 32) shrink_mma_kernel(const bf16* __re
   constexpr int N = (16 * MT + 31) / 32, STAGE = shrink_stage<MT, NJ>();
   Adapters<N> adapters;
 #pragma unroll
-  for (int i = 0; i < N; ++i) adapters.id[i] = 32 * i + lane < 16 * MT ? ids[32 * i + lane] : -1;
-  adapters.start();
+  for (int i = 0; i < N; ++i) { adapters.id[i] = 32 * i + lane < 16 * MT ? ids[32 * i + lane] : -1; adapters.high[i] = 0; }
+  adapters.start(rows.n);
   const uint32_t mine = smem_u32(ring) + warp * STAGES * STAGE;
   const int blocks = (cols + 63) / 64, n = blocks > warp ? (blocks - warp + WARPS - 1) / WARPS : 0;      // blocks of columns, and this warp's of them
   float* part = reinterpret_cast<float*>(ring);        // [warps][16 MT][8 NJ]
@@ -166,9 +183,11 @@ __global__ void __launch_bounds__(WARPS * 32) shrink_mma_kernel(const bf16* __re
 // from L2 for W, which is what bounds the product: with a 128 x 256 tile to one SM every 128 x 256 x 64 step fetched 48 KB, 12 TB/s over the
 // chip, and ran at 46 % of the tensor cores' rate (9216 rows 1024 -> 4096 without adapters: 89.9 us).
 //
-// Warp 0 fetches tiles of x and W by TMA into a ring of stages, warps 2..5 fill the stages of the adapters' steps by hand, warp 1 (of the
-// pair's first CTA) issues the products, warps 6..9 drain one accumulator (tensor memory, bias, bf16, shared memory, whole 128-byte lines)
-// while the other one fills.  All of them walk the same list of steps; warp 10 counts the adapters of the worker's tiles ahead of the others.
+// Warp 0 fetches tiles of x and W by TMA into a ring of stages, warps 2..5 fill two stages of their own with the adapters' tiles, warp 1 (of
+// the pair's first CTA) issues the products, warps 6..9 drain one accumulator (tensor memory, bias, bf16, shared memory, TMA) while the other one
+// fills.  Warp 10 counts the adapters of the worker's tiles ahead of the others.  The adapters have stages apart because a load takes as long as
+// all that TMA has asked for before it, 2500 cycles: filled a tile ahead they cost the product nothing, in the ring 4 us a tile (9216
+// rows 1024 -> 4096, one adapter: 90 us, without 54).
 //
 // 0 x NaN is NaN, so what an adapter holds must not meet other rows' zeros: numbers that are not finite are left out of the B tile, and the
 // rows of that adapter get their products from a loop at the end.
@@ -176,8 +195,9 @@ constexpr int BM = 128, THREADS = 352, MOST_TILES = 512;   // MOST_TILES: of one
 constexpr uint32_t A_BYTES = BM * 128;
 constexpr uint64_t WAIT_NS = 1000ull * 1000ull * 1000ull;
 __host__ __device__ constexpr uint32_t stage_bytes(int bn, int ctas) { return A_BYTES + (uint32_t)(bn / ctas) * 128; }
-__host__ __device__ constexpr int stages_of(int bn, int ctas) { return 192 * 1024 / (int)stage_bytes(bn, ctas); }
-__host__ __device__ constexpr uint32_t ring_bytes(int bn, int ctas) { return (uint32_t)stages_of(bn, ctas) * stage_bytes(bn, ctas); }
+constexpr int AHEAD = 2;                               // stages of the adapters
+__host__ __device__ constexpr int stages_of(int bn, int ctas) { return 192 * 1024 / (int)stage_bytes(bn, ctas) - AHEAD; }
+__host__ __device__ constexpr uint32_t ring_bytes(int bn, int ctas) { return (uint32_t)(stages_of(bn, ctas) + AHEAD) * stage_bytes(bn, ctas); }
 constexpr uint32_t OUT_BYTES = 2 * 4 * 32 * 128, BAR_BYTES = 512 + 2 * MOST_TILES;
 __host__ __device__ constexpr uint32_t smem_of(int bn, int ctas) { return ring_bytes(bn, ctas) + OUT_BYTES + BAR_BYTES + 1024; }
 
@@ -267,10 +287,8 @@ __device__ __forceinline__ void free_columns(uint32_t tmem, uint32_t n) {
 // W along its other axis: groups of 64 columns, each 64 rows of 128 bytes (rows run along the inner dimension).
 __device__ __forceinline__ uint64_t smem_desc_columns(uint32_t saddr) { return (smem_desc_sw128(saddr) & ~(0x3FFFull << 16)) | ((uint64_t)(8192 >> 4) << 16); }
 
-// Eight factors of one output column from j on.
-template <bool VEC>
+// Eight factors of one output column from j on, where they are not vectors.
 __device__ __forceinline__ uint4 factors8(const bf16* row, int j, int rank) {
-  if (VEC) return j < rank ? __ldg(reinterpret_cast<const uint4*>(row + j)) : make_uint4(0, 0, 0, 0);
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -309,10 +327,10 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
   constexpr uint32_t BARS = ring_bytes(BN, CTAS) + OUT_BYTES;
-  // full[s] (the first CTA's counts for both), empty[s], granted[s], then for both accumulators: filled, drained
+  // full[s] (the first CTA's counts for both CTAs) and empty[s], the adapters' stages behind the others; then for both accumulators: filled, drained
   auto bar = [&](int i) { return base + BARS + 8u * (uint32_t)i; };
-  constexpr int EMPTY = S, GRANTED = 2 * S, FILLED = 3 * S, DRAINED = 3 * S + 2;
-  static_assert(8 * (3 * S + 4) <= 256, "barriers");
+  constexpr int EMPTY = S + AHEAD, FILLED = 2 * EMPTY, DRAINED = FILLED + 2;
+  static_assert(8 * (DRAINED + 2) <= 256, "barriers");
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + BARS + 256);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + BARS + 260);
   volatile int* counted = reinterpret_cast<volatile int*>(gbase + BARS + 268);                 // tiles whose adapters have been counted
@@ -325,7 +343,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
     *abort_flag = 0;
     *bad_factors = 0;
     *counted = 0;
-    for (int i = 0; i < 3 * S; ++i) mbar_init(bar(i), i < S ? CTAS : 1u);
+    for (int i = 0; i < 2 * EMPTY; ++i) mbar_init(bar(i), i < EMPTY ? CTAS : 1u);
     for (int i = 0; i < 2; ++i) { mbar_init(bar(FILLED + i), 1u); mbar_init(bar(DRAINED + i), 4u * CTAS); }
     fence_mbar_init();
     prefetch_tmap(&tm_x);
@@ -359,15 +377,14 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
   auto tile_row = [&](int tile) { return (int64_t)(tile / n_tiles) * BM * CTAS; };
 
   // Stages go round; `odd` is the parity of the round.  A fresh barrier counts as having completed the phase before its first.
-  int s = 0, odd = 0;
+  int s = 0, odd = 0, extra = 0, extra_odd = 0;
   auto advance = [&] { if (++s == S) { s = 0; odd ^= 1; } };
+  auto advance_extra = [&] { if (++extra == AHEAD) { extra = 0; extra_odd ^= 1; } };
 
   if (warp == 0) {
     // ---- tiles of x and W
-    for (int tile = worker; tile < tiles; tile += workers, ++it) {
+    for (int tile = worker; tile < tiles; tile += workers) {
       const int m0 = (int)tile_row(tile) + rank * BM, n0 = tile % n_tiles * BN + rank * PART;
-      // Lane 0 alone waits for stages, in the order of the steps, and grants those of the adapters' steps to the warps that fill them: a
-      // barrier tells two neighbouring phases apart and no more, so nobody may wait for one that others can go past.
       if (lane == 0) {
         bool go = true;
         for (int k = 0; k < nk; ++k, advance()) {
@@ -383,11 +400,6 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
 #pragma unroll
             for (int c = 0; c < PART / 64; ++c) tma_load_2d<CTAS>(b + c * 8192, &tm_w, full, n0 + c * 64, k * 64);
           }
-        }
-        const int more = (count_of(it) * inner + 63) / 64;
-        for (int k = 0; k < more; ++k, advance()) {
-          wait(EMPTY + s, odd ^ 1);
-          mbar_arrive(bar(GRANTED + s));
         }
       }
       __syncwarp();
@@ -410,91 +422,111 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
         for (int i = 1; i < 4; ++i) mma_step<CTAS>(acc, a + 2 * i, b + ALONG * i, ID, 1u);
         commit_step<CTAS>(bar(EMPTY + s));
       }
-      for (int left = count_of(it) * inner; left > 0; left -= 64, advance()) {
-        wait(s, odd);
+      for (int left = count_of(it) * inner; left > 0; left -= 64, advance_extra()) {
+        wait(S + extra, extra_odd);
         tc_fence_after();
-        const uint64_t a = a0 + (uint32_t)s * (STAGE >> 4), b = b0 + (uint32_t)s * (STAGE >> 4);
+        const uint64_t a = a0 + (uint32_t)(S + extra) * (STAGE >> 4), b = b0 + (uint32_t)(S + extra) * (STAGE >> 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (16 * i < left) mma_step<CTAS>(acc, a + 2 * i, b + 2 * i, ID_ADAPTERS, 1u);
-        commit_step<CTAS>(bar(EMPTY + s));
+        commit_step<CTAS>(bar(EMPTY + S + extra));
       }
       commit_step<CTAS>(bar(FILLED + (it & 1)));
     }
   } else if (warp >= 2 && warp < 6) {
-    // ---- the adapters' steps: h as the A tile, with zeros in the rows of other adapters, and B_a as the B tile
-    const int w = warp - 2, me = w * 32 + lane;
-    uint32_t grants = 0;                               // of each stage: the phase to wait for
+    // ---- the adapters' steps: h as the A tile, with zeros in the rows of other adapters, and B_a as the B tile.  Two warps to each of the two
+    // stages, so that one is on its way while the other is checked, handed over or waited for.
+    static_assert(AHEAD == 2, "two pairs of warps");
+    const int stage = S + (warp - 2) / 2, half = warp & 1;       // rows 32 half + lane, and those 64 further on, of both tiles
+    constexpr int BR = PART / 64;
+    uint32_t bad = 0;
+    auto copy = [](uint32_t dst, const void* src, bool real) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+    };
+    const int me = half * 32 + lane;
+    const uint32_t at = base + stage * STAGE + me * 128;
+    auto place = [&](int r, int piece) { return at + r * 64 * 128 + ((piece ^ (me & 7)) << 4); };
     Tile adapters;
+    if (worker < tiles) adapters.ask(p.rows, tile_row(worker), lane);
     wait_for_stream();                                 // hx is made by the kernel in front
     for (int tile = worker; tile < tiles; tile += workers, ++it) {
-      const int64_t row0 = tile_row(tile);
+      const bf16* h = p.hx + (tile_row(tile) + rank * BM + me) * inner;
       const int n0 = tile % n_tiles * BN + rank * PART;
-      adapters.load(p.rows, row0, lane);
-      adapters.start();
-      int mine = -1;                                   // of row `me` of this CTA's rows
+      adapters.start(p.rows.n);
+      int mine[2] = {-1, -1};
 #pragma unroll
       for (int i = 0; i < 4 * CTAS; ++i)
-        if (i == (int)rank * 4 + w) mine = adapters.id[i];
-      s = (s + nk) % S;
-      uint32_t bad = 0;
-      const uint4* h = reinterpret_cast<const uint4*>(p.hx + (row0 + rank * BM + me) * inner);
-      const int left = count_of(it) * inner / 8;       // pieces of eight columns
-      int a = -1, q = 0;                               // the adapter, and the column of it, that the next piece is
-      for (int first = 0; first < left; first += 8, advance()) {
-        const int pieces = min(8, left - first);
-        constexpr int BR = (PART + 127) / 128;
-        uint4 av[8], bv[BR][8];                        // both tiles are on their way before the stage is free
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const bool in = i < pieces;
-          if (in && q == 0) a = adapters.next();
-          av[i] = in && mine == a ? h[q / 8] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-          for (int r = 0; r < BR; ++r) {
-            const bool real = in && me + 128 * r < PART && n0 + me + 128 * r < p.N;
-            bv[r][i] = real ? factors8<VEC>(p.f + ((int64_t)a * p.N + n0 + me + 128 * r) * p.rank, q >= p.r16 ? q - p.r16 : q, p.rank) : make_uint4(0, 0, 0, 0);
-          }
-          if (in) q = q + 8 == inner ? 0 : q + 8;
+        if (i / 4 == (int)rank && i % 2 == half) mine[i % 4 / 2] = adapters.id[i];
+      int a = -1, q = inner;                           // the adapter, and the column of it, that comes next
+      for (int left = count_of(it) * inner / 8; left > 0; left -= 8, advance_extra()) {        // left: pieces of eight columns
+        const int pieces = min(8, left);
+        const bool ours = S + extra == stage;
+        if (ours) {
+          if (lane == 0) wait(EMPTY + stage, extra_odd ^ 1);
+          __syncwarp();
         }
+#pragma unroll
+        for (int four = 0; four < 8; four += 4) {      // an adapter has a multiple of four pieces
+          if (four >= pieces) break;
+          if (q == inner) { a = adapters.next(); q = 0; }
+          if (ours) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) copy(place(r, four + i), mine[r] == a ? h + (int64_t)r * 64 * inner + q + 8 * i : p.hx, mine[r] == a);
+#pragma unroll
+            for (int r = 0; r < BR; ++r) {
+              const int n = n0 + me + 64 * r;
+              const bf16* row = p.f + ((int64_t)a * p.N + min(n, p.N - 1)) * p.rank;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int j = q + 8 * i >= p.r16 ? q + 8 * i - p.r16 : q + 8 * i;
+                const bool real = n < p.N && j < p.rank;
+                if (VEC) {
+                  copy(place(r, four + i) + A_BYTES, real ? row + j : p.f, real);
+                } else {
+                  const uint4 v = factors8(row, j, real ? p.rank : 0);
+                  sts_128(place(r, four + i) + A_BYTES, v.x, v.y, v.z, v.w);
+                }
+              }
+            }
+          }
+          q += 32;
+        }
+        if (!ours) continue;
+        asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
         for (int r = 0; r < BR; ++r)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) bv[r][i] = finite8(bv[r][i], bad);
-        if (lane == 0) wait(GRANTED + s, (int)(grants >> s));
-        __syncwarp();
-        grants ^= 1u << s;
-        const uint32_t at = base + s * STAGE;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (i >= pieces) break;
-          sts_128(at + me * 128 + ((i ^ (me & 7)) << 4), av[i].x, av[i].y, av[i].z, av[i].w);
-#pragma unroll
-          for (int r = 0; r < BR; ++r) {
-            const uint4& v = bv[r][i];
-            if (PART >= 128 || me < PART) sts_128(at + A_BYTES + (me + 128 * r) * 128 + ((i ^ (me & 7)) << 4), v.x, v.y, v.z, v.w);
+          for (int i = 0; i < 8; ++i) {
+            if (i >= pieces) break;
+            uint32_t worse = 0;
+            const uint4 v = finite8(lds_128(place(r, i) + A_BYTES), worse);
+            if (worse) sts_128(place(r, i) + A_BYTES, v.x, v.y, v.z, v.w);
+            bad |= worse;
           }
-        }
         fence_proxy_async_smem();
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync %0, 64;" ::"r"(stage - S + 1) : "memory");
         if (me == 0) {
-          if (CTAS == 2) arrive_in_cluster<true>(in_cta(bar(s), 0));
-          else mbar_arrive(bar(s));
+          if (CTAS == 2) arrive_in_cluster<true>(in_cta(bar(stage), 0));
+          else mbar_arrive(bar(stage));
         }
       }
-      if (bad) {                                       // for the loop at the end, in both CTAs
-        const uint32_t at = smem_u32(const_cast<uint32_t*>(bad_factors));
-        if (CTAS == 1) *bad_factors = 1;
-        else
-          for (int r = 0; r < CTAS; ++r) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_cta(at, r)), "r"(1u) : "memory");
-      }
-      __syncwarp();
+      if (tile + workers < tiles) adapters.ask(p.rows, tile_row(tile + workers), lane);
     }
+    if (bad) {                                         // for the loop at the end, in both CTAs
+      const uint32_t at = smem_u32(const_cast<uint32_t*>(bad_factors));
+      if (CTAS == 1) *bad_factors = 1;
+      else
+        for (int r = 0; r < CTAS; ++r) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_cta(at, r)), "r"(1u) : "memory");
+    }
+    __syncwarp();
   } else if (warp == 10) {
     // ---- how many adapters each tile has
     for (int tile = worker; tile < tiles; tile += workers, ++it) {
       Tile adapters;
-      adapters.load(p.rows, tile_row(tile), lane);
+      adapters.ask(p.rows, tile_row(tile), lane);
+      adapters.start(p.rows.n);
       const int n = adapters.count();
       if (lane == 0) {
         counts[it] = (uint16_t)n;
