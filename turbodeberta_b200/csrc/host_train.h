@@ -278,16 +278,15 @@ struct LoraCall {
   }
 };
 
-// The inner values of the rows: bf16 [rows, inner] from the tensor cores, else fp32 [shares, rows, rank].  f: the factors, for the former.
+// The inner values of the rows: bf16 [rows, inner] from the tensor cores, else fp32 [rows, rank].  f: the factors, for the former.
 Tensor lora_shrink(const LoraCall& c, bool back, const Tensor& f, cudaStream_t stream) {
   Tensor h;
   if (c.tensor_cores) {
     h = at::empty({c.l.rows, tdb_lora_inner(&c.l)}, c.w.options());
     check_rc(tdb_lora_umma_shrink(&c.l, back, f.data_ptr(), h.data_ptr(), stream));
   } else {
-    const int shares = tdb_lora_shares(&c.l, back);
-    h = c.floats({shares, c.l.rows, c.l.rank});
-    check_rc(tdb_lora_shrink(&c.l, back, h.data_ptr<float>(), shares, stream));
+    h = c.floats({c.l.rows, c.l.rank});
+    check_rc(tdb_lora_shrink(&c.l, back, h.data_ptr<float>(), stream));
   }
   return h;
 }
@@ -303,16 +302,9 @@ Tensor lora_product(const LoraCall& c, bool back, const Tensor& f, const Tensor&
   }
   const Tensor base = back ? c.product(c.dy.t, c.w) : c.product(c.x.t, c.w.t());
   Tensor y = c.l.dtype == TDB_DTYPE_F32 ? base : at::empty({c.l.rows, cols}, c.w.options());
-  check_rc(tdb_lora_expand(&c.l, back, base.data_ptr<float>(), h.data_ptr<float>(), (int)h.size(0), y.data_ptr(), stream.stream()));
+  check_rc(tdb_lora_expand(&c.l, back, base.data_ptr<float>(), h.data_ptr<float>(), y.data_ptr(), stream.stream()));
   return y;
 }
-// [n, r, c] -> [n, c, r]
-Tensor lora_turned(const Tensor& t, cudaStream_t stream) {
-  Tensor out = at::empty({t.size(0), t.size(2), t.size(1)}, t.options());
-  check_rc(tdb_lora_turn(t.data_ptr(), (int)t.size(0), (int)t.size(1), (int)t.size(2), out.data_ptr(), stream));
-  return out;
-}
-
 // y, and the rows' inner values, from which the gradient of b is made.
 std::pair<Tensor, Tensor> run_lora(LoraCall& c, at::IntArrayRef shape) {
   const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream();
@@ -324,10 +316,10 @@ std::pair<Tensor, Tensor> run_lora(LoraCall& c, at::IntArrayRef shape) {
 Tensor lora_gradient(const LoraCall& c, bool of_b, const Tensor& v, cudaStream_t stream) {
   const Tensor& like = of_b ? c.b : c.a;
   if (c.l.rows == 0) return at::zeros_like(like);
-  const int shares = tdb_lora_gather_shares(&c.l, of_b);
+  const int shares = tdb_lora_gather_shares(&c.l, of_b, c.tensor_cores ? tdb_lora_umma_gather_factors(&c.l) : 16);
   Tensor part = c.floats({shares, c.l.n, c.l.rank, of_b ? c.l.features : c.l.cols}), out = at::empty(like.sizes(), like.options());
   if (c.tensor_cores) check_rc(tdb_lora_umma_gather(&c.l, of_b, v.data_ptr(), part.data_ptr<float>(), shares, stream));
-  else check_rc(tdb_lora_gather(&c.l, of_b, v.data_ptr<float>(), (int)v.size(0), part.data_ptr<float>(), shares, stream));
+  else check_rc(tdb_lora_gather(&c.l, of_b, v.data_ptr<float>(), part.data_ptr<float>(), shares, stream));
   check_rc(tdb_lora_gather_sum(&c.l, of_b, part.data_ptr<float>(), shares, out.data_ptr(), stream));
   return out;
 }
@@ -361,7 +353,12 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
       if (need_x) dx = at::empty(x.sizes(), x.options());
     } else if (need_x || need_a) {
       // the product may start beside the kernel in front of it, which therefore is the one that makes u
-      const Tensor a_turned = c.tensor_cores && need_x ? lora_turned(c.a, stream) : Tensor(), b_turned = c.tensor_cores ? lora_turned(c.b, stream) : Tensor();
+      Tensor a_turned, b_turned;
+      if (c.tensor_cores) {
+        if (need_x) a_turned = at::empty({c.l.n, c.l.cols, c.l.rank}, a.options());
+        b_turned = at::empty({c.l.n, c.l.rank, c.l.features}, b.options());
+        check_rc(tdb_lora_turn(&c.l, need_x ? a_turned.data_ptr() : nullptr, b_turned.data_ptr(), stream));
+      }
       u = lora_shrink(c, true, b_turned, stream);
       if (need_x) dx = lora_product(c, true, a_turned, u, stream).view(x.sizes());
     }

@@ -18,77 +18,92 @@ __device__ __forceinline__ float value(const __nv_bfloat16* p) { return __bfloat
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-constexpr int TILE = 16, COLS = 128, STEP = 64;
+constexpr int TILE = 16, COLS = 128;
 
 // One matrix per adapter, factor j of column c at j * sj + c * sc.
 template <typename T> struct Factors { const T* p; int64_t each, sj, sc; };
 
-// The rows' adapters in shared memory; whether `row` is the first of its adapter in the tile.
-__device__ __forceinline__ void load_ids(int* ids, const LoraRows& rows, int64_t t0, int count) {
-  if ((int)threadIdx.x < count) ids[threadIdx.x] = t0 + threadIdx.x < rows.rows ? adapter_of(rows, t0 + threadIdx.x) : -1;
+// The adapters of up to 32 rows, and which of them there are, by the block's first warp.
+struct Present { int id[32], list[32], count; };
+__device__ __forceinline__ void find_present(Present& s, const LoraRows& rows, int64_t t0, int n) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x, id = lane < n && t0 + lane < rows.rows ? adapter_of(rows, t0 + lane) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, id);
+    const bool first = id >= 0 && (same & ((1u << lane) - 1u)) == 0;
+    const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+    s.id[lane] = id;
+    if (first) s.list[__popc(firsts & ((1u << lane) - 1u))] = id;
+    if (lane == 0) s.count = __popc(firsts);
+  }
   __syncthreads();
 }
-__device__ __forceinline__ bool is_first(const int* ids, int row) {
-  for (int i = 0; i < row; ++i)
-    if (ids[i] == ids[row]) return false;
-  return true;
-}
 
-// h[z][t][j] = s_a sum over this share of the columns of x[t][c] F_a(j, c).  A block: 16 rows, 64 factors.
+// h[t][j] = s_a sum over the columns of x[t][c] F_a(j, c).  A block: four rows; its warps share the columns, eight factors at a time, so that a
+// thread's 12 loads feed 32 products.  Bound by the factors' way through the first-level cache.
+constexpr int S_ROWS = 4, S_WARPS = 8, S_FACTORS = 8;
 template <typename T>
-__global__ void __launch_bounds__(256) shrink_kernel(const T* __restrict__ x, int64_t stride, int cols, Factors<T> f, int rank, LoraRows rows,
-                                                     int share, float* __restrict__ h) {
-  __shared__ int ids[TILE];
-  __shared__ float xs[TILE][STEP + 1], fs[STEP][64 + 1];
-  const int64_t t0 = (int64_t)blockIdx.x * TILE;
-  const int j0 = blockIdx.y * 64, jn = min(64, rank - j0), c_begin = blockIdx.z * share, c_end = min(cols, c_begin + share);
-  const int row = threadIdx.x / 16, jt = threadIdx.x % 16;              // a thread: one row, factors jt, jt + 16, ...
-  load_ids(ids, rows, t0, TILE);
-  float out[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int first = 0; first < TILE; ++first) {
-    const int a = ids[first];
-    if (a < 0 || !is_first(ids, first)) continue;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c0 = c_begin; c0 < c_end; c0 += STEP) {
-      __syncthreads();
-      for (int e = threadIdx.x; e < TILE * STEP; e += 256) {
-        const int r = e / STEP, c = e % STEP;
-        xs[r][c] = ids[r] == a && c0 + c < c_end ? value(x + (t0 + r) * stride + c0 + c) : 0.f;
-      }
-      const T* fa = f.p + a * f.each;
-      for (int e = threadIdx.x; e < STEP * 64; e += 256) {
-        const int j = f.sj == 1 ? e % 64 : e / STEP, c = f.sj == 1 ? e / 64 : e % STEP;
-        fs[c][j] = j < jn && c0 + c < c_end ? value(fa + (j0 + j) * f.sj + (int64_t)(c0 + c) * f.sc) : 0.f;
-      }
-      __syncthreads();
-      if (ids[row] == a) {
-        for (int c = 0; c < STEP; ++c) {
-          const float v = xs[row][c];
+__global__ void __launch_bounds__(S_WARPS * 32) shrink_kernel(const T* __restrict__ x, int64_t stride, int cols, Factors<T> f, int rank, LoraRows rows,
+                                                             float* __restrict__ h) {
+  __shared__ Present here;
+  __shared__ float part[S_WARPS][S_ROWS * S_FACTORS];
+  const int64_t t0 = (int64_t)blockIdx.x * S_ROWS;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, j0 = blockIdx.y * S_FACTORS;
+  find_present(here, rows, t0, S_ROWS);
+  for (int k = 0; k < here.count; ++k) {
+    const int a = here.list[k];
+    const T* fa = f.p + a * f.each + j0 * f.sj;
+    float acc[S_ROWS][S_FACTORS];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] = fmaf(v, fs[c][jt + 16 * i], acc[i]);
-        }
-      }
+    for (int r = 0; r < S_ROWS; ++r)
+#pragma unroll
+      for (int j = 0; j < S_FACTORS; ++j) acc[r][j] = 0.f;
+#pragma unroll 2
+    for (int c = threadIdx.x; c < cols; c += S_WARPS * 32) {
+      float xv[S_ROWS], fv[S_FACTORS];
+#pragma unroll
+      for (int r = 0; r < S_ROWS; ++r) xv[r] = here.id[r] == a ? value(x + (t0 + r) * stride + c) : 0.f;
+#pragma unroll
+      for (int j = 0; j < S_FACTORS; ++j) fv[j] = j0 + j < rank ? value(fa + j * f.sj + (int64_t)c * f.sc) : 0.f;
+#pragma unroll
+      for (int r = 0; r < S_ROWS; ++r)
+#pragma unroll
+        for (int j = 0; j < S_FACTORS; ++j) acc[r][j] = fmaf(xv[r], fv[j], acc[r][j]);
     }
-    if (ids[row] == a) {
+    // 32 sums over 32 lanes: lanes trade halves, and lane l ends with sum l
+    float v[32];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) out[i] = acc[i] * scaling_of(rows, a);
+    for (int i = 0; i < 32; ++i) v[i] = acc[i / S_FACTORS][i % S_FACTORS];
+#pragma unroll
+    for (int half = 16; half >= 1; half >>= 1) {
+      const bool up = lane & half;
+#pragma unroll
+      for (int i = 0; i < half; ++i) v[i] = (up ? v[i + half] : v[i]) + __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + half], half);
+    }
+    __syncthreads();
+    part[warp][lane] = v[0];
+    __syncthreads();
+    if (warp == 0) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < S_WARPS; ++w) s += part[w][lane];
+      const int r = lane / S_FACTORS, j = j0 + lane % S_FACTORS;
+      if (here.id[r] == a && j < rank) h[(t0 + r) * rank + j] = s * scaling_of(rows, a);
     }
   }
-  if (t0 + row >= rows.rows) return;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (jt + 16 * i < jn) h[((int64_t)blockIdx.z * rows.rows + t0 + row) * rank + j0 + jt + 16 * i] = out[i];
 }
 
 // y[t][c] = base[t][c] + bias[c] + sum over j of h[t][j] F_a(j, c), one rounding.  A block: 16 rows, 128 columns, one to a thread.
 template <typename T>
-__global__ void __launch_bounds__(COLS) expand_kernel(const float* base, const T* __restrict__ bias, const float* __restrict__ h, int shares,
-                                                      int rank, Factors<T> f, LoraRows rows, int cols, T* y) {     // base may be y
-  __shared__ int ids[TILE];
+__global__ void __launch_bounds__(COLS) expand_kernel(const float* base, const T* __restrict__ bias, const float* __restrict__ h, int rank, Factors<T> f,
+                                                      LoraRows rows, int cols, T* y) {     // base may be y
+  __shared__ Present here;
   __shared__ float hs[TILE][64];
   const int64_t t0 = (int64_t)blockIdx.x * TILE;
   const int c = blockIdx.y * COLS + threadIdx.x;
-  load_ids(ids, rows, t0, TILE);
+  float sum[TILE];                                   // on their way while the rows' adapters are looked up
+#pragma unroll
+  for (int r = 0; r < TILE; ++r) sum[r] = c < cols && t0 + r < rows.rows ? base[(t0 + r) * cols + c] : 0.f;
+  find_present(here, rows, t0, TILE);
   float acc[TILE];
 #pragma unroll
   for (int r = 0; r < TILE; ++r) acc[r] = 0.f;
@@ -97,24 +112,21 @@ __global__ void __launch_bounds__(COLS) expand_kernel(const float* base, const T
     __syncthreads();
     for (int e = threadIdx.x; e < TILE * 64; e += COLS) {
       const int r = e / 64, j = e % 64;
-      float s = 0.f;
-      if (j < jn && ids[r] >= 0)
-        for (int z = 0; z < shares; ++z) s += h[((int64_t)z * rows.rows + t0 + r) * rank + j0 + j];
-      hs[r][j] = s;
+      hs[r][j] = j < jn && here.id[r] >= 0 ? h[(t0 + r) * rank + j0 + j] : 0.f;
     }
     __syncthreads();
     if (c >= cols) continue;
-    for (int first = 0; first < TILE; ++first) {
-      const int a = ids[first];
-      if (a < 0 || !is_first(ids, first)) continue;
+    for (int k = 0; k < here.count; ++k) {
+      const int a = here.list[k];
       const T* fa = f.p + a * f.each + j0 * f.sj + (int64_t)c * f.sc;
-      bool mine[TILE];
+      uint32_t mine = 0;
 #pragma unroll
-      for (int r = 0; r < TILE; ++r) mine[r] = ids[r] == a;
+      for (int r = 0; r < TILE; ++r) mine |= (here.id[r] == a ? 1u : 0u) << r;
+#pragma unroll 4
       for (int j = 0; j < jn; ++j) {
         const float v = value(fa + j * f.sj);
 #pragma unroll
-        for (int r = 0; r < TILE; ++r) acc[r] = mine[r] ? fmaf(hs[r][j], v, acc[r]) : acc[r];
+        for (int r = 0; r < TILE; ++r) acc[r] = mine >> r & 1 ? fmaf(hs[r][j], v, acc[r]) : acc[r];
       }
     }
   }
@@ -122,12 +134,12 @@ __global__ void __launch_bounds__(COLS) expand_kernel(const float* base, const T
   const float b = bias ? value(bias + c) : 0.f;
 #pragma unroll
   for (int r = 0; r < TILE; ++r)
-    if (t0 + r < rows.rows) put(y + (t0 + r) * cols + c, base[(t0 + r) * cols + c] + b + acc[r]);
+    if (t0 + r < rows.rows) put(y + (t0 + r) * cols + c, sum[r] + b + acc[r]);
 }
 
 // part[z][a][j][c] = sum over this share of the rows t of adapter a of v[t][j] x[t][c].  A block: one adapter, 16 factors, 128 columns.
 template <typename T>
-__global__ void __launch_bounds__(COLS) gather_kernel(const T* __restrict__ x, int64_t stride, int cols, const float* __restrict__ v, int shares, int rank,
+__global__ void __launch_bounds__(COLS) gather_kernel(const T* __restrict__ x, int64_t stride, int cols, const float* __restrict__ v, int rank,
                                                       LoraRows rows, int64_t share, int j_blocks, float* __restrict__ part) {
   __shared__ int ids[32];
   __shared__ float vs[32][16];
@@ -144,21 +156,20 @@ __global__ void __launch_bounds__(COLS) gather_kernel(const T* __restrict__ x, i
     if (!__syncthreads_or(mine)) continue;
     for (int e = threadIdx.x; e < 32 * 16; e += COLS) {
       const int r = e / 16, j = e % 16;
-      float s = 0.f;
-      if (ids[r] && j < jn)
-        for (int z = 0; z < shares; ++z) s += v[((int64_t)z * rows.rows + t0 + r) * rank + j0 + j];
-      vs[r][j] = s;
+      vs[r][j] = ids[r] && j < jn ? v[(t0 + r) * rank + j0 + j] : 0.f;
     }
-    __syncthreads();
-    if (c < cols) {
-#pragma unroll 8
-      for (int r = 0; r < 32; ++r) {
-        if (!ids[r]) continue;
-        const float xv = value(x + (t0 + r) * stride + c);
+    float xv[32];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) acc[j] = fmaf(vs[r][j], xv, acc[j]);
+    for (int r = 0; r < 32; ++r) xv[r] = ids[r] && c < cols ? value(x + (t0 + r) * stride + c) : 0.f;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(&vs[r][j]);
+        acc[j] = fmaf(q.x, xv[r], acc[j]); acc[j + 1] = fmaf(q.y, xv[r], acc[j + 1]);
+        acc[j + 2] = fmaf(q.z, xv[r], acc[j + 2]); acc[j + 3] = fmaf(q.w, xv[r], acc[j + 3]);
       }
-    }
   }
   if (c >= cols) return;
   const int n = gridDim.y / j_blocks;
@@ -167,44 +178,60 @@ __global__ void __launch_bounds__(COLS) gather_kernel(const T* __restrict__ x, i
     if (j < jn) part[(((int64_t)blockIdx.z * n + a) * rank + j0 + j) * cols + c] = acc[j];
 }
 
-// The shares' sum, as [a][j][c] or, turned, [a][c][j].
-template <typename T, bool TURNED>
-__global__ void __launch_bounds__(256) gather_sum_kernel(const float* __restrict__ part, int shares, int64_t total, int rank, int cols, T* __restrict__ out) {
+// The shares' sum, as [a][j][c] or, turned by squares of 32, [a][c][j].
+template <typename T>
+__global__ void __launch_bounds__(256) gather_sum_kernel(const float* __restrict__ part, int shares, int64_t total, T* __restrict__ out) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (e >= total) return;
-  int64_t from = e;
-  if (TURNED) {
-    const int64_t j = e % rank, c = e / rank % cols, a = e / rank / cols;
-    from = (a * rank + j) * cols + c;
-  }
   float s = 0.f;
-  for (int z = 0; z < shares; ++z) s += part[z * total + from];
+#pragma unroll 8
+  for (int z = 0; z < shares; ++z) s += part[z * total + e];
   put(out + e, s);
+}
+template <typename T>
+__global__ void __launch_bounds__(256) gather_sum_turned_kernel(const float* __restrict__ part, int shares, int64_t total, int rank, int cols, T* __restrict__ out) {
+  __shared__ float s[32][33];
+  const int64_t a = blockIdx.z;
+  const int c0 = blockIdx.x * 32, j0 = blockIdx.y * 32, tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+#pragma unroll
+  for (int i = ty; i < 32; i += 8) {
+    float v = 0.f;
+    if (j0 + i < rank && c0 + tx < cols)
+#pragma unroll 8
+      for (int z = 0; z < shares; ++z) v += part[z * total + (a * rank + j0 + i) * cols + c0 + tx];
+    s[i][tx] = v;
+  }
+  __syncthreads();
+  const int wide = min(32, rank - j0);               // neighbouring threads write neighbouring factors, whatever the rank
+  for (int e = threadIdx.x; e < 32 * wide; e += 256) {
+    const int c = e / wide, j = e % wide;
+    if (c0 + c < cols) put(out + (a * cols + c0 + c) * rank + j0 + j, s[j][c]);
+  }
 }
 
 LoraRows rows_of(const Lora& l) { return LoraRows{l.ids, l.id_bytes, l.rows_per_id, l.rows, l.n, l.scaling, l.scaling_value}; }
 
 template <typename T>
-int shrink(const Lora& l, bool back, float* h, int shares, cudaStream_t s) {
-  const int cols = back ? l.features : l.cols, share = (cols + shares - 1) / shares;
+int shrink(const Lora& l, bool back, float* h, cudaStream_t s) {
+  const int cols = back ? l.features : l.cols;
   const Factors<T> f = back ? Factors<T>{(const T*)l.b, (int64_t)l.features * l.rank, 1, l.rank} : Factors<T>{(const T*)l.a, (int64_t)l.cols * l.rank, l.cols, 1};
-  const dim3 grid((unsigned)((l.rows + TILE - 1) / TILE), (l.rank + 63) / 64, shares);
-  shrink_kernel<T><<<grid, 256, 0, s>>>((const T*)(back ? l.dy : l.x), back ? l.dy_stride : l.x_stride, cols, f, l.rank, rows_of(l), share, h);
+  const dim3 grid((unsigned)((l.rows + S_ROWS - 1) / S_ROWS), (l.rank + S_FACTORS - 1) / S_FACTORS);
+  shrink_kernel<T><<<grid, S_WARPS * 32, 0, s>>>((const T*)(back ? l.dy : l.x), back ? l.dy_stride : l.x_stride, cols, f, l.rank, rows_of(l), h);
   return cuda_fail(cudaGetLastError(), "lora shrink launch");
 }
 template <typename T>
-int expand(const Lora& l, bool back, const float* base, const float* h, int shares, void* y, cudaStream_t s) {
+int expand(const Lora& l, bool back, const float* base, const float* h, void* y, cudaStream_t s) {
   const int cols = back ? l.cols : l.features;
   const Factors<T> f = back ? Factors<T>{(const T*)l.a, (int64_t)l.cols * l.rank, l.cols, 1} : Factors<T>{(const T*)l.b, (int64_t)l.features * l.rank, 1, l.rank};
   const dim3 grid((unsigned)((l.rows + TILE - 1) / TILE), (cols + COLS - 1) / COLS);
-  expand_kernel<T><<<grid, COLS, 0, s>>>(base, back ? nullptr : (const T*)l.bias, h, shares, l.rank, f, rows_of(l), cols, (T*)y);
+  expand_kernel<T><<<grid, COLS, 0, s>>>(base, back ? nullptr : (const T*)l.bias, h, l.rank, f, rows_of(l), cols, (T*)y);
   return cuda_fail(cudaGetLastError(), "lora expand launch");
 }
 template <typename T>
-int gather(const Lora& l, bool of_b, const float* v, int v_shares, float* part, int shares, cudaStream_t s) {
+int gather(const Lora& l, bool of_b, const float* v, float* part, int shares, cudaStream_t s) {
   const int cols = of_b ? l.features : l.cols, j_blocks = (l.rank + 15) / 16;
   const dim3 grid((cols + COLS - 1) / COLS, l.n * j_blocks, shares);
-  gather_kernel<T><<<grid, COLS, 0, s>>>((const T*)(of_b ? l.dy : l.x), of_b ? l.dy_stride : l.x_stride, cols, v, v_shares, l.rank, rows_of(l),
+  gather_kernel<T><<<grid, COLS, 0, s>>>((const T*)(of_b ? l.dy : l.x), of_b ? l.dy_stride : l.x_stride, cols, v, l.rank, rows_of(l),
                                          (l.rows + shares - 1) / shares, j_blocks, part);
   return cuda_fail(cudaGetLastError(), "lora gather launch");
 }
@@ -212,9 +239,8 @@ template <typename T>
 int gather_sum(const Lora& l, bool of_b, const float* part, int shares, void* out, cudaStream_t s) {
   const int cols = of_b ? l.features : l.cols;
   const int64_t total = (int64_t)l.n * l.rank * cols;
-  const unsigned blocks = (unsigned)((total + 255) / 256);
-  if (of_b) gather_sum_kernel<T, true><<<blocks, 256, 0, s>>>(part, shares, total, l.rank, cols, (T*)out);
-  else gather_sum_kernel<T, false><<<blocks, 256, 0, s>>>(part, shares, total, l.rank, cols, (T*)out);
+  if (of_b) gather_sum_turned_kernel<T><<<dim3((cols + 31) / 32, (l.rank + 31) / 32, l.n), 256, 0, s>>>(part, shares, total, l.rank, cols, (T*)out);
+  else gather_sum_kernel<T><<<(unsigned)((total + 255) / 256), 256, 0, s>>>(part, shares, total, (T*)out);
   return cuda_fail(cudaGetLastError(), "lora gather sum launch");
 }
 
@@ -225,32 +251,22 @@ using namespace tdb;
 
 extern "C" {
 
-// Few rows leave SMs idle, so their columns are shared out, down to 256 columns a block; `expand` and `gather` add the shares up.
-int tdb_lora_shares(const Lora* l, int back) {
+// How many parts the rows of a gradient are shared out in, so that there are four blocks to an SM, down to 64 rows a part.  factors: to a block.
+int tdb_lora_gather_shares(const Lora* l, int of_b, int factors) {
   int sms = 0;
   if (device_sms(&sms)) return 1;
-  const int cols = back ? l->features : l->cols;
-  const int64_t blocks = (l->rows + TILE - 1) / TILE * ((l->rank + 63) / 64);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(cols + 255) / 256, sms / std::max<int64_t>(1, blocks), 8}));
-}
-// Likewise for the rows of a gradient, down to 128 of them a block.
-int tdb_lora_gather_shares(const Lora* l, int of_b) {
-  int sms = 0;
-  if (device_sms(&sms)) return 1;
-  const int64_t blocks = (int64_t)l->n * ((l->rank + 15) / 16) * (((of_b ? l->features : l->cols) + COLS - 1) / COLS);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(l->rows + 127) / 128, 4 * sms / std::max<int64_t>(1, blocks), 32}));
+  const int64_t blocks = (int64_t)l->n * ((l->rank + factors - 1) / factors) * (((of_b ? l->features : l->cols) + COLS - 1) / COLS);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(l->rows + 63) / 64, 4 * sms / std::max<int64_t>(1, blocks), 32}));
 }
 
-int tdb_lora_shrink(const Lora* l, int back, float* h, int shares, void* stream) {
-  return l->dtype == TDB_DTYPE_F32 ? shrink<float>(*l, back, h, shares, (cudaStream_t)stream) : shrink<__nv_bfloat16>(*l, back, h, shares, (cudaStream_t)stream);
+int tdb_lora_shrink(const Lora* l, int back, float* h, void* stream) {
+  return l->dtype == TDB_DTYPE_F32 ? shrink<float>(*l, back, h, (cudaStream_t)stream) : shrink<__nv_bfloat16>(*l, back, h, (cudaStream_t)stream);
 }
-int tdb_lora_expand(const Lora* l, int back, const float* base, const float* h, int shares, void* y, void* stream) {
-  return l->dtype == TDB_DTYPE_F32 ? expand<float>(*l, back, base, h, shares, y, (cudaStream_t)stream)
-                                   : expand<__nv_bfloat16>(*l, back, base, h, shares, y, (cudaStream_t)stream);
+int tdb_lora_expand(const Lora* l, int back, const float* base, const float* h, void* y, void* stream) {
+  return l->dtype == TDB_DTYPE_F32 ? expand<float>(*l, back, base, h, y, (cudaStream_t)stream) : expand<__nv_bfloat16>(*l, back, base, h, y, (cudaStream_t)stream);
 }
-int tdb_lora_gather(const Lora* l, int of_b, const float* v, int v_shares, float* part, int shares, void* stream) {
-  return l->dtype == TDB_DTYPE_F32 ? gather<float>(*l, of_b, v, v_shares, part, shares, (cudaStream_t)stream)
-                                   : gather<__nv_bfloat16>(*l, of_b, v, v_shares, part, shares, (cudaStream_t)stream);
+int tdb_lora_gather(const Lora* l, int of_b, const float* v, float* part, int shares, void* stream) {
+  return l->dtype == TDB_DTYPE_F32 ? gather<float>(*l, of_b, v, part, shares, (cudaStream_t)stream) : gather<__nv_bfloat16>(*l, of_b, v, part, shares, (cudaStream_t)stream);
 }
 int tdb_lora_gather_sum(const Lora* l, int of_b, const float* part, int shares, void* out, void* stream) {
   return l->dtype == TDB_DTYPE_F32 ? gather_sum<float>(*l, of_b, part, shares, out, (cudaStream_t)stream)

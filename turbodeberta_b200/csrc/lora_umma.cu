@@ -734,16 +734,24 @@ __global__ void __launch_bounds__(256) gather_mma_kernel(const bf16* __restrict_
     }
 }
 
-// in [n][rows][cols] -> out [n][cols][rows], by squares of 32
-__global__ void __launch_bounds__(256) turn_kernel(const bf16* __restrict__ in, int rows, int cols, bf16* __restrict__ out) {
+// [n][rows][cols] -> [n][cols][rows] by squares of 32, for two lists of matrices at once.
+struct Turn { const bf16* in; bf16* out; int rows, cols, blocks; };       // blocks: of one matrix
+__global__ void __launch_bounds__(256) turn_kernel(Turn first, Turn second) {
   __shared__ bf16 s[32][33];
-  const int64_t at = (int64_t)blockIdx.z * rows * cols;
-  const int c0 = blockIdx.x * 32, r0 = blockIdx.y * 32, tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  const bool later = (int)blockIdx.x >= first.blocks;
+  const Turn& t = later ? second : first;
+  const int64_t at = (int64_t)blockIdx.y * t.rows * t.cols;
+  const int block = blockIdx.x - (later ? first.blocks : 0), across = (t.cols + 31) / 32;
+  const int c0 = block % across * 32, r0 = block / across * 32, tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+#pragma unroll
   for (int i = ty; i < 32; i += 8)
-    if (r0 + i < rows && c0 + tx < cols) s[i][tx] = in[at + (int64_t)(r0 + i) * cols + c0 + tx];
+    if (r0 + i < t.rows && c0 + tx < t.cols) s[i][tx] = t.in[at + (int64_t)(r0 + i) * t.cols + c0 + tx];
   __syncthreads();
-  for (int i = ty; i < 32; i += 8)
-    if (c0 + i < cols && r0 + tx < rows) out[at + (int64_t)(c0 + i) * rows + r0 + tx] = s[tx][i];
+  const int wide = min(32, t.rows - r0);
+  for (int e = threadIdx.x; e < 32 * wide; e += 256) {
+    const int c = e / wide, r = e % wide;
+    if (c0 + c < t.cols) t.out[at + (int64_t)(c0 + c) * t.rows + r0 + r] = s[r][c];
+  }
 }
 
 LoraRows rows_of(const Lora& l) { return LoraRows{l.ids, l.id_bytes, l.rows_per_id, l.rows, l.n, l.scaling, l.scaling_value}; }
@@ -838,13 +846,19 @@ int tdb_lora_umma_product(const Lora* l, int back, const void* f, const void* hx
   return run(shape.columns == 256 ? launch_product<256, 2, false> : shape.columns == 128 ? launch_product<128, 1, false> : launch_product<64, 1, false>);
 }
 
-int tdb_lora_turn(const void* in, int n, int rows, int cols, void* out, void* stream) {
-  turn_kernel<<<dim3((cols + 31) / 32, (rows + 31) / 32, n), 256, 0, (cudaStream_t)stream>>>((const bf16*)in, rows, cols, (bf16*)out);
+int tdb_lora_turn(const Lora* l, void* a_turned, void* b_turned, void* stream) {
+  auto list = [](const void* in, void* out, int rows, int cols) {
+    return Turn{(const bf16*)in, (bf16*)out, rows, cols, out ? (cols + 31) / 32 * ((rows + 31) / 32) : 0};
+  };
+  const Turn a = list(l->a, a_turned, l->rank, l->cols), b = list(l->b, b_turned, l->features, l->rank);
+  turn_kernel<<<dim3(a.blocks + b.blocks, l->n), 256, 0, (cudaStream_t)stream>>>(a, b);
   return cuda_fail(cudaGetLastError(), "lora turn launch");
 }
 
+int tdb_lora_umma_gather_factors(const Lora* l) { return l->rank <= 16 ? 16 : l->rank <= 32 ? 32 : 64; }
+
 int tdb_lora_umma_gather(const Lora* l, int of_b, const void* v, float* part, int shares, void* stream) {
-  const int cols = of_b ? l->features : l->cols, r16 = r16_of(*l), mt = r16 <= 16 ? 1 : r16 <= 32 ? 2 : 4, j_blocks = (r16 + 16 * mt - 1) / (16 * mt);
+  const int cols = of_b ? l->features : l->cols, r16 = r16_of(*l), mt = tdb_lora_umma_gather_factors(l) / 16, j_blocks = (r16 + 16 * mt - 1) / (16 * mt);
   const int64_t share = ((l->rows + shares - 1) / shares + 63) / 64 * 64;
   auto run = [&](auto kernel) {
     if (const int rc = opt_in_smem(reinterpret_cast<const void*>(kernel), gather_smem(mt))) return rc;

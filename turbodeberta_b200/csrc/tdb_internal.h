@@ -195,14 +195,13 @@ TDB_HOST_API int tdb_dropout(const void* x, void* y, int64_t n, int dtype, const
 TDB_HOST_API int tdb_norm_forward(const tdb::Norm* n, int dtype, void* stream);
 TDB_HOST_API int64_t tdb_norm_partial_floats(int64_t rows, int cols);
 TDB_HOST_API int tdb_norm_backward(const tdb::Norm* n, int dtype, void* stream);
-// Adapters beside a shared product, any type and size.  back: from dy through b and a instead of from x through a and b.  h: [shares, rows, rank], the
-// shares to be added up.  base: the product alone, fp32 [rows, columns of y].
-TDB_HOST_API int tdb_lora_shares(const tdb::Lora* l, int back);
-TDB_HOST_API int tdb_lora_shrink(const tdb::Lora* l, int back, float* h, int shares, void* stream);
-TDB_HOST_API int tdb_lora_expand(const tdb::Lora* l, int back, const float* base, const float* h, int shares, void* y, void* stream);
-// The gradient of a (from v = u and x) or of b (from v = h and dy).  part: [shares, n, rank, columns] floats.
-TDB_HOST_API int tdb_lora_gather_shares(const tdb::Lora* l, int of_b);
-TDB_HOST_API int tdb_lora_gather(const tdb::Lora* l, int of_b, const float* v, int v_shares, float* part, int shares, void* stream);
+// Adapters beside a shared product, any type and size.  back: from dy through b and a instead of from x through a and b.  h: fp32 [rows, rank].
+// base: the product alone, fp32 [rows, columns of y].
+TDB_HOST_API int tdb_lora_shrink(const tdb::Lora* l, int back, float* h, void* stream);
+TDB_HOST_API int tdb_lora_expand(const tdb::Lora* l, int back, const float* base, const float* h, void* y, void* stream);
+// The gradient of a (from v = u and x) or of b (from v = h and dy).  part: [shares, n, rank, columns] floats.  factors: of a block, 16 here.
+TDB_HOST_API int tdb_lora_gather_shares(const tdb::Lora* l, int of_b, int factors);
+TDB_HOST_API int tdb_lora_gather(const tdb::Lora* l, int of_b, const float* v, float* part, int shares, void* stream);
 // The sum of gather's shares, to the type and layout of a (or of b).
 TDB_HOST_API int tdb_lora_gather_sum(const tdb::Lora* l, int of_b, const float* part, int shares, void* out, void* stream);
 // The same on the tensor cores (lora_umma.cu), for bf16 with columns and features that are multiples of eight, all tensors 16-byte aligned and rows no
@@ -213,5 +212,7 @@ TDB_HOST_API int64_t tdb_lora_inner(const tdb::Lora* l);
 TDB_HOST_API int tdb_lora_umma_shrink(const tdb::Lora* l, int back, const void* f, void* hx, void* stream);
 TDB_HOST_API int tdb_lora_umma_product(const tdb::Lora* l, int back, const void* f, const void* hx, void* y, int32_t* status, void* stream);
 TDB_HOST_API int tdb_lora_umma_gather(const tdb::Lora* l, int of_b, const void* v, float* part, int shares, void* stream);
-TDB_HOST_API int tdb_lora_turn(const void* in, int n, int rows, int cols, void* out, void* stream);
+// a and b turned, either to null where it is not needed.
+TDB_HOST_API int tdb_lora_turn(const tdb::Lora* l, void* a_turned, void* b_turned, void* stream);
+TDB_HOST_API int tdb_lora_umma_gather_factors(const tdb::Lora* l);
 }
