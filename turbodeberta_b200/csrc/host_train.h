@@ -279,11 +279,11 @@ struct LoraCall {
 };
 
 // The inner values of the rows: bf16 [rows, inner] from the tensor cores, else fp32 [rows, rank].  f: the factors, for the former.
-Tensor lora_shrink(const LoraCall& c, bool back, const Tensor& f, cudaStream_t stream) {
+Tensor lora_shrink(const LoraCall& c, bool back, const Tensor& f, cudaStream_t stream, const Tensor& owners = {}) {
   Tensor h;
   if (c.tensor_cores) {
     h = at::empty({c.l.rows, tdb_lora_inner(&c.l)}, c.w.options());
-    check_rc(tdb_lora_umma_shrink(&c.l, back, f.data_ptr(), h.data_ptr(), stream));
+    check_rc(tdb_lora_umma_shrink(&c.l, back, f.data_ptr(), h.data_ptr(), owners.defined() ? static_cast<uint16_t*>(owners.data_ptr()) : nullptr, stream));
   } else {
     h = c.floats({c.l.rows, c.l.rank});
     check_rc(tdb_lora_shrink(&c.l, back, h.data_ptr<float>(), stream));
@@ -305,20 +305,22 @@ Tensor lora_product(const LoraCall& c, bool back, const Tensor& f, const Tensor&
   check_rc(tdb_lora_expand(&c.l, back, base.data_ptr<float>(), h.data_ptr<float>(), y.data_ptr(), stream.stream()));
   return y;
 }
-// y, and the rows' inner values, from which the gradient of b is made.
-std::pair<Tensor, Tensor> run_lora(LoraCall& c, at::IntArrayRef shape) {
+// y; the rows' inner values, from which the gradient of b is made; and, where the tensor cores will make gradients, which row is whose.
+std::tuple<Tensor, Tensor, Tensor> run_lora(LoraCall& c, at::IntArrayRef shape, bool train) {
   const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream();
-  if (c.l.rows == 0) return {at::empty(shape, c.w.options()), Tensor()};
-  const Tensor h = lora_shrink(c, false, c.a, stream);
-  return {lora_product(c, false, c.b, h, stream).view(shape), h};
+  if (c.l.rows == 0) return {at::empty(shape, c.w.options()), Tensor(), Tensor()};
+  Tensor owners;
+  if (train && c.tensor_cores) owners = at::empty({(c.l.rows + 15) / 16, c.l.n}, c.w.options().dtype(at::kShort));
+  const Tensor h = lora_shrink(c, false, c.a, stream, owners);
+  return {lora_product(c, false, c.b, h, stream).view(shape), h, owners};
 }
 
-Tensor lora_gradient(const LoraCall& c, bool of_b, const Tensor& v, cudaStream_t stream) {
+Tensor lora_gradient(const LoraCall& c, bool of_b, const Tensor& v, const Tensor& owners, cudaStream_t stream) {
   const Tensor& like = of_b ? c.b : c.a;
   if (c.l.rows == 0) return at::zeros_like(like);
   const int shares = tdb_lora_gather_shares(&c.l, of_b, c.tensor_cores ? tdb_lora_umma_gather_factors(&c.l) : 16);
   Tensor part = c.floats({shares, c.l.n, c.l.rank, of_b ? c.l.features : c.l.cols}), out = at::empty(like.sizes(), like.options());
-  if (c.tensor_cores) check_rc(tdb_lora_umma_gather(&c.l, of_b, v.data_ptr(), part.data_ptr<float>(), shares, stream));
+  if (c.tensor_cores) check_rc(tdb_lora_umma_gather(&c.l, of_b, v.data_ptr(), static_cast<const uint16_t*>(owners.data_ptr()), part.data_ptr<float>(), shares, stream));
   else check_rc(tdb_lora_gather(&c.l, of_b, v.data_ptr<float>(), part.data_ptr<float>(), shares, stream));
   check_rc(tdb_lora_gather_sum(&c.l, of_b, part.data_ptr<float>(), shares, out.data_ptr(), stream));
   return out;
@@ -331,8 +333,8 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
     at::AutoDispatchBelowAutograd below;
     c10::cuda::CUDAGuard guard(x.device());
     LoraCall c(x, w, bias, a, b, scaling, scaling_value, ids);
-    auto [y, h] = run_lora(c, shape);
-    ctx->save_for_backward({x, w, a, b, scaling ? *scaling : Tensor(), ids ? *ids : Tensor(), b.requires_grad() ? h : Tensor()});
+    auto [y, h, owners] = run_lora(c, shape, a.requires_grad() || b.requires_grad());
+    ctx->save_for_backward({x, w, a, b, scaling ? *scaling : Tensor(), ids ? *ids : Tensor(), b.requires_grad() ? h : Tensor(), owners});
     ctx->saved_data["scaling"] = scaling_value;
     ctx->saved_data["bias"] = bias.has_value();
     return y;
@@ -340,7 +342,7 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     refuse_second_derivative("lora_linear");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &a = saved[2], &b = saved[3], &scaling = saved[4], &ids = saved[5], &h = saved[6];
+    const Tensor &x = saved[0], &w = saved[1], &a = saved[2], &b = saved[3], &scaling = saved[4], &ids = saved[5], &h = saved[6], &owners = saved[7];
     const int at = ctx->saved_data["bias"].toBool() ? 3 : 2;
     const bool need_x = ctx->needs_input_grad(0), need_a = ctx->needs_input_grad(at), need_b = ctx->needs_input_grad(at + 1);
     c10::cuda::CUDAGuard guard(x.device());
@@ -362,8 +364,8 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
       u = lora_shrink(c, true, b_turned, stream);
       if (need_x) dx = lora_product(c, true, a_turned, u, stream).view(x.sizes());
     }
-    if (need_a) da = lora_gradient(c, false, u, stream);
-    if (need_b) db = lora_gradient(c, true, h, stream);
+    if (need_a) da = lora_gradient(c, false, u, owners, stream);
+    if (need_b) db = lora_gradient(c, true, h, owners, stream);
     const Tensor none;
     return {dx, none, none, da, db, none, none, none, none};
   }
@@ -402,5 +404,5 @@ Tensor lora_linear(const Tensor& x, const Tensor& w, const OptTensor& bias, cons
   }
   c10::cuda::CUDAGuard guard(x.device());
   LoraCall c(x, w, bias, a, b, scaling, scaling_value, ids);
-  return run_lora(c, shape).first;
+  return std::get<0>(run_lora(c, shape, false));
 }

@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(COLS) gather_kernel(const T* __restrict__ x, i
     if (j < jn) part[(((int64_t)blockIdx.z * n + a) * rank + j0 + j) * cols + c] = acc[j];
 }
 
-// The shares' sum, as [a][j][c] or, turned by squares of 32, [a][c][j].
+// The shares' sum, as [a][j][c] or, turned by pieces of 8 x 32, [a][c][j].
 template <typename T>
 __global__ void __launch_bounds__(256) gather_sum_kernel(const float* __restrict__ part, int shares, int64_t total, T* __restrict__ out) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -190,23 +190,17 @@ __global__ void __launch_bounds__(256) gather_sum_kernel(const float* __restrict
 }
 template <typename T>
 __global__ void __launch_bounds__(256) gather_sum_turned_kernel(const float* __restrict__ part, int shares, int64_t total, int rank, int cols, T* __restrict__ out) {
-  __shared__ float s[32][33];
+  __shared__ float s[8][33];
   const int64_t a = blockIdx.z;
-  const int c0 = blockIdx.x * 32, j0 = blockIdx.y * 32, tx = threadIdx.x % 32, ty = threadIdx.x / 32;
-#pragma unroll
-  for (int i = ty; i < 32; i += 8) {
-    float v = 0.f;
-    if (j0 + i < rank && c0 + tx < cols)
+  const int c0 = blockIdx.x * 32, j0 = blockIdx.y * 8, tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  float v = 0.f;
+  if (j0 + ty < rank && c0 + tx < cols)
 #pragma unroll 8
-      for (int z = 0; z < shares; ++z) v += part[z * total + (a * rank + j0 + i) * cols + c0 + tx];
-    s[i][tx] = v;
-  }
+    for (int z = 0; z < shares; ++z) v += part[z * total + (a * rank + j0 + ty) * cols + c0 + tx];
+  s[ty][tx] = v;
   __syncthreads();
-  const int wide = min(32, rank - j0);               // neighbouring threads write neighbouring factors, whatever the rank
-  for (int e = threadIdx.x; e < 32 * wide; e += 256) {
-    const int c = e / wide, j = e % wide;
-    if (c0 + c < cols) put(out + (a * cols + c0 + c) * rank + j0 + j, s[j][c]);
-  }
+  const int c = threadIdx.x / 8, j = threadIdx.x % 8;
+  if (j0 + j < rank && c0 + c < cols) put(out + (a * cols + c0 + c) * rank + j0 + j, s[j][c]);
 }
 
 LoraRows rows_of(const Lora& l) { return LoraRows{l.ids, l.id_bytes, l.rows_per_id, l.rows, l.n, l.scaling, l.scaling_value}; }
@@ -239,7 +233,7 @@ template <typename T>
 int gather_sum(const Lora& l, bool of_b, const float* part, int shares, void* out, cudaStream_t s) {
   const int cols = of_b ? l.features : l.cols;
   const int64_t total = (int64_t)l.n * l.rank * cols;
-  if (of_b) gather_sum_turned_kernel<T><<<dim3((cols + 31) / 32, (l.rank + 31) / 32, l.n), 256, 0, s>>>(part, shares, total, l.rank, cols, (T*)out);
+  if (of_b) gather_sum_turned_kernel<T><<<dim3((cols + 31) / 32, (l.rank + 7) / 8, l.n), 256, 0, s>>>(part, shares, total, l.rank, cols, (T*)out);
   else gather_sum_kernel<T><<<(unsigned)((total + 255) / 256), 256, 0, s>>>(part, shares, total, (T*)out);
   return cuda_fail(cudaGetLastError(), "lora gather sum launch");
 }

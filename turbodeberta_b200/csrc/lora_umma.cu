@@ -75,12 +75,12 @@ struct Adapters {
 // hx[t] = the inner values of row t: r16 high parts, r16 low parts.  A block: 16 MT rows and 8 NJ factors; its warps share the columns, blocks of
 // 64 in turn, and add up through shared memory.  Bound by reading x, and the factors from L2 once for every block: each warp has STAGES blocks
 // of columns on their way into shared memory that is its own, so that nothing waits for the block's other warps.
-// blockIdx.z takes every gridDim.z-th adapter of the rows.
+// blockIdx.z takes every gridDim.z-th adapter of the rows.  owners [rows / 16][n], where it is wanted: for the gradients, which of the rows are whose.
 template <int MT, int NJ> __host__ __device__ constexpr int shrink_stage() { return (16 * MT + 8 * NJ) * 128; }
 
 template <int MT, int NJ, int WARPS, int STAGES>
 __global__ void __launch_bounds__(WARPS * 32) shrink_mma_kernel(const bf16* __restrict__ x, int64_t stride, int cols, const bf16* __restrict__ f, int rank,
-                                                                int r16, LoraRows rows, bf16* __restrict__ hx) {
+                                                                int r16, LoraRows rows, bf16* __restrict__ hx, uint16_t* __restrict__ owners) {
   extern __shared__ __align__(128) uint8_t ring[];     // [warps][stages][rows of x, then factors][64]; then the warps' sums
   __shared__ int ids[16 * MT];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4, j0 = blockIdx.y * 8 * NJ;
@@ -93,6 +93,15 @@ __global__ void __launch_bounds__(WARPS * 32) shrink_mma_kernel(const bf16* __re
 #pragma unroll
   for (int i = 0; i < N; ++i) { adapters.id[i] = 32 * i + lane < 16 * MT ? ids[32 * i + lane] : -1; adapters.high[i] = 0; }
   adapters.start(rows.n);
+  if (owners && blockIdx.y == 0 && blockIdx.z == 0)    // which of sixteen rows are an adapter's, for every adapter
+    for (int e = threadIdx.x; e < MT * rows.n; e += WARPS * 32) {
+      const int m = e / rows.n, a = e % rows.n;
+      if (t0 + 16 * m >= rows.rows) break;
+      uint32_t mask = 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mask |= (ids[16 * m + r] == a ? 1u : 0u) << r;
+      owners[((t0 >> 4) + m) * rows.n + a] = (uint16_t)mask;
+    }
   const uint32_t mine = smem_u32(ring) + warp * STAGES * STAGE;
   const int blocks = (cols + 63) / 64, n = blocks > warp ? (blocks - warp + WARPS - 1) / WARPS : 0;      // blocks of columns, and this warp's of them
   float* part = reinterpret_cast<float*>(ring);        // [warps][16 MT][8 NJ]
@@ -630,23 +639,25 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
 }
 
 // ------------------------------------------------------------------------------------------------------------------- gather
-// part[z][a][j][c] = sum over this share of the rows t of adapter a of v[t][j] x[t][c], v being the sum of two bf16 numbers.  A block: one
+// part[z][a][j][c] = sum over a share of the rows t of adapter a of v[t][j] x[t][c], v being the sum of two bf16 numbers.  A block: one
 // adapter, 16 MT factors, 128 columns; a warp: 16 columns.  Rows come in tiles of 64 through shared memory, two at a time; tiles without
-// a row of the adapter are passed over, and other rows of a tile are zeros in both operands.  Bound by reading x.
+// a row of the adapter are passed over, and other rows of a tile are zeros in both operands.  Of the tiles with one, blockIdx.z takes every
+// gridDim.z-th: ranges of rows would leave most blocks without work where requests are long (8192 rows, four adapters: 46 us).  Bound by reading x.
 constexpr int GC = 128, GP = GC + 8, G_BATCH = 256;
 __host__ __device__ constexpr int gather_pitch(int mt) { return 32 * mt + 8; }
 __host__ __device__ constexpr int gather_smem(int mt) { return 2 * 64 * (GP + gather_pitch(mt)) * 2; }
 
 template <int MT>
 __global__ void __launch_bounds__(256) gather_mma_kernel(const bf16* __restrict__ x, int64_t stride, int cols, const bf16* __restrict__ v, int r16, int rank,
-                                                         LoraRows rows, int64_t share, int j_blocks, float* __restrict__ part) {
+                                                         const uint16_t* __restrict__ owners, int64_t rows, int n_adapters, int j_blocks, float* __restrict__ part) {
   constexpr int VP = gather_pitch(MT);
   extern __shared__ __align__(16) bf16 tiles[];
   __shared__ uint64_t masks[G_BATCH];
+  __shared__ int list[G_BATCH], listed;
   bf16 *xs[2] = {tiles, tiles + 64 * GP}, *vs[2] = {tiles + 2 * 64 * GP, tiles + 2 * 64 * GP + 64 * VP};
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int a = blockIdx.y / j_blocks, j0 = blockIdx.y % j_blocks * 16 * MT, c0 = blockIdx.x * GC;
-  const int64_t begin = blockIdx.z * share, end = min(rows.rows, begin + share);
+  uint32_t seen = 0;                                   // tiles with a row of the adapter so far
   float acc[MT][2][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -658,22 +669,32 @@ __global__ void __launch_bounds__(256) gather_mma_kernel(const bf16* __restrict_
   auto copy = [](bf16* dst, const bf16* src, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(saddr(dst)), "l"(src), "r"(real ? 16 : 0) : "memory");
   };
-  for (int64_t batch = begin; batch < end; batch += 64 * G_BATCH) {
-    const int n = (int)min((int64_t)G_BATCH, (end - batch + 63) / 64);
+  for (int64_t batch = 0; batch < rows; batch += 64 * G_BATCH) {
+    const int n = (int)min((int64_t)G_BATCH, (rows - batch + 63) / 64);
     __syncthreads();
-#pragma unroll 4
-    for (int i = warp; i < n; i += 8) {
-      const int64_t t = batch + 64 * i + lane;
-      const uint32_t lo = __ballot_sync(0xffffffffu, t < end && adapter_of(rows, t) == a);
-      const uint32_t hi = __ballot_sync(0xffffffffu, t + 32 < end && adapter_of(rows, t + 32) == a);
-      if (lane == 0) masks[i] = (uint64_t)hi << 32 | lo;
+    if (tid < n) {
+      uint64_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (batch + 64 * tid + 16 * i < rows) m |= (uint64_t)owners[((batch >> 4) + 4 * tid + i) * n_adapters + a] << (16 * i);
+      masks[tid] = m;
     }
     __syncthreads();
-    auto next = [&](int i) {
-      do ++i;
-      while (i < n && masks[i] == 0);
-      return i;
-    };
+    if (warp == 0) {
+      int mine = 0;
+      for (int i0 = 0; i0 < n; i0 += 32) {
+        const bool any = i0 + lane < n && masks[i0 + lane] != 0;
+        const uint32_t with = __ballot_sync(0xffffffffu, any), before = (1u << lane) - 1u;
+        const bool ours = any && (seen + __popc(with & before)) % gridDim.z == blockIdx.z;
+        const uint32_t all = __ballot_sync(0xffffffffu, ours);
+        if (ours) list[mine + __popc(all & before)] = i0 + lane;
+        mine += __popc(all);
+        seen += __popc(with);
+      }
+      if (lane == 0) listed = mine;
+    }
+    __syncthreads();
+    const int todo = listed;
     auto load = [&](int i, int buf) {
       const uint64_t m = masks[i];
       const int64_t t0 = batch + 64 * i;
@@ -691,13 +712,14 @@ __global__ void __launch_bounds__(256) gather_mma_kernel(const bf16* __restrict_
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    int i = next(-1), buf = 0;
-    if (i < n) load(i, 0);
-    while (i < n) {
-      const int then = next(i);
-      if (then < n) load(then, buf ^ 1);
-      if (then < n) asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (todo > 0) load(list[0], 0);
+    for (int i = 0, buf = 0; i < todo; ++i, buf ^= 1) {
+      if (i + 1 < todo) {
+        load(list[i + 1], buf ^ 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      } else {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+      }
       __syncthreads();
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -714,11 +736,9 @@ __global__ void __launch_bounds__(256) gather_mma_kernel(const bf16* __restrict_
           }
       }
       __syncthreads();
-      i = then;
-      buf ^= 1;
     }
   }
-  const int n = gridDim.y / j_blocks, g = lane / 4, t = lane % 4;
+  const int g = lane / 4, t = lane % 4;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -729,7 +749,7 @@ __global__ void __launch_bounds__(256) gather_mma_kernel(const bf16* __restrict_
       for (int e = 0; e < 2; ++e) {
         const int c = c0 + warp * 16 + 8 * e + 2 * t;
         if (c < cols)
-          *reinterpret_cast<float2*>(part + (((int64_t)blockIdx.z * n + a) * rank + j) * cols + c) = make_float2(acc[m][e][2 * r], acc[m][e][2 * r + 1]);
+          *reinterpret_cast<float2*>(part + (((int64_t)blockIdx.z * n_adapters + a) * rank + j) * cols + c) = make_float2(acc[m][e][2 * r], acc[m][e][2 * r + 1]);
       }
     }
 }
@@ -758,7 +778,7 @@ LoraRows rows_of(const Lora& l) { return LoraRows{l.ids, l.id_bytes, l.rows_per_
 int r16_of(const Lora& l) { return (l.rank + 15) / 16 * 16; }
 
 template <int MT, int NJ, int WARPS, int STAGES>
-int launch_shrink(const Lora& l, const bf16* x, int64_t stride, int cols, const bf16* f, bf16* hx, int sms, cudaStream_t s) {
+int launch_shrink(const Lora& l, const bf16* x, int64_t stride, int cols, const bf16* f, bf16* hx, uint16_t* owners, int sms, cudaStream_t s) {
   constexpr int smem = WARPS * STAGES * shrink_stage<MT, NJ>();
   static_assert(WARPS * 16 * MT * 8 * NJ * 4 <= smem, "the warps' sums");
   auto kernel = shrink_mma_kernel<MT, NJ, WARPS, STAGES>;
@@ -767,7 +787,7 @@ int launch_shrink(const Lora& l, const bf16* x, int64_t stride, int cols, const 
   const int js = (r16_of(l) + 8 * NJ - 1) / (8 * NJ);
   // where there are SMs to spare, a tile's adapters are shared out too
   const int z = (int)std::max<int64_t>(1, std::min<int64_t>({l.n, 16 * MT, l.rows, 2 * sms / std::max<int64_t>(1, tiles * js)}));
-  kernel<<<dim3((unsigned)tiles, js, z), WARPS * 32, smem, s>>>(x, stride, cols, f, l.rank, r16_of(l), rows_of(l), hx);
+  kernel<<<dim3((unsigned)tiles, js, z), WARPS * 32, smem, s>>>(x, stride, cols, f, l.rank, r16_of(l), rows_of(l), hx, owners);
   return cuda_fail(cudaGetLastError(), "lora shrink launch");
 }
 
@@ -817,13 +837,13 @@ int tdb_lora_umma_applies(const Lora* l) {
 
 int64_t tdb_lora_inner(const Lora* l) { return 2 * r16_of(*l); }
 
-int tdb_lora_umma_shrink(const Lora* l, int back, const void* f, void* hx, void* stream) {
+int tdb_lora_umma_shrink(const Lora* l, int back, const void* f, void* hx, uint16_t* owners, void* stream) {
   int sms = 0;
   if (const int rc = device_sms(&sms)) return rc;
   const bf16* x = (const bf16*)(back ? l->dy : l->x);
   const int64_t stride = back ? l->dy_stride : l->x_stride;
   const int cols = back ? l->features : l->cols;
-  auto run = [&](auto launch) { return launch(*l, x, stride, cols, (const bf16*)f, (bf16*)hx, sms, (cudaStream_t)stream); };
+  auto run = [&](auto launch) { return launch(*l, x, stride, cols, (const bf16*)f, (bf16*)hx, owners, sms, (cudaStream_t)stream); };
   const bool few = l->rows <= 16 * sms;
   if (l->rank <= 16) return run(few ? launch_shrink<1, 2, 8, 2> : launch_shrink<2, 2, 4, 4>);
   if (l->rank <= 32) return run(few ? launch_shrink<1, 4, 8, 2> : launch_shrink<2, 4, 4, 3>);
@@ -857,13 +877,12 @@ int tdb_lora_turn(const Lora* l, void* a_turned, void* b_turned, void* stream) {
 
 int tdb_lora_umma_gather_factors(const Lora* l) { return l->rank <= 16 ? 16 : l->rank <= 32 ? 32 : 64; }
 
-int tdb_lora_umma_gather(const Lora* l, int of_b, const void* v, float* part, int shares, void* stream) {
+int tdb_lora_umma_gather(const Lora* l, int of_b, const void* v, const uint16_t* owners, float* part, int shares, void* stream) {
   const int cols = of_b ? l->features : l->cols, r16 = r16_of(*l), mt = tdb_lora_umma_gather_factors(l) / 16, j_blocks = (r16 + 16 * mt - 1) / (16 * mt);
-  const int64_t share = ((l->rows + shares - 1) / shares + 63) / 64 * 64;
   auto run = [&](auto kernel) {
     if (const int rc = opt_in_smem(reinterpret_cast<const void*>(kernel), gather_smem(mt))) return rc;
     kernel<<<dim3((cols + GC - 1) / GC, l->n * j_blocks, shares), 256, gather_smem(mt), (cudaStream_t)stream>>>(
-        (const bf16*)(of_b ? l->dy : l->x), of_b ? l->dy_stride : l->x_stride, cols, (const bf16*)v, r16, l->rank, rows_of(*l), share, j_blocks, part);
+        (const bf16*)(of_b ? l->dy : l->x), of_b ? l->dy_stride : l->x_stride, cols, (const bf16*)v, r16, l->rank, owners, l->rows, l->n, j_blocks, part);
     return cuda_fail(cudaGetLastError(), "lora gather launch");
   };
   return mt == 1 ? run(gather_mma_kernel<1>) : mt == 2 ? run(gather_mma_kernel<2>) : run(gather_mma_kernel<4>);

@@ -207,11 +207,12 @@ TDB_HOST_API int tdb_lora_gather_sum(const tdb::Lora* l, int of_b, const float* 
 // The same on the tensor cores (lora_umma.cu), for bf16 with columns and features that are multiples of eight, all tensors 16-byte aligned and rows no
 // less than a row apart.  f: the factors that are multiplied with x (a) or dy (b turned, [n, rank, features]) in `shrink`, and those that make y (b) or dx (a
 // turned, [n, cols, rank]) in `product`.  hx, v: bf16 [rows, tdb_lora_inner()].  status: int32[4], word 0 tells of a wait that gave up.
+// owners: [ceil(rows / 16)][n], written by `shrink` unless null, read by `gather`.
 TDB_HOST_API int tdb_lora_umma_applies(const tdb::Lora* l);
 TDB_HOST_API int64_t tdb_lora_inner(const tdb::Lora* l);
-TDB_HOST_API int tdb_lora_umma_shrink(const tdb::Lora* l, int back, const void* f, void* hx, void* stream);
+TDB_HOST_API int tdb_lora_umma_shrink(const tdb::Lora* l, int back, const void* f, void* hx, uint16_t* owners, void* stream);
 TDB_HOST_API int tdb_lora_umma_product(const tdb::Lora* l, int back, const void* f, const void* hx, void* y, int32_t* status, void* stream);
-TDB_HOST_API int tdb_lora_umma_gather(const tdb::Lora* l, int of_b, const void* v, float* part, int shares, void* stream);
+TDB_HOST_API int tdb_lora_umma_gather(const tdb::Lora* l, int of_b, const void* v, const uint16_t* owners, float* part, int shares, void* stream);
 // a and b turned, either to null where it is not needed.
 TDB_HOST_API int tdb_lora_turn(const tdb::Lora* l, void* a_turned, void* b_turned, void* stream);
 TDB_HOST_API int tdb_lora_umma_gather_factors(const tdb::Lora* l);
