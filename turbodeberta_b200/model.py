@@ -29,7 +29,9 @@ from transformers.models.deberta_v2.modeling_deberta_v2 import (
     DebertaV2Intermediate, DebertaV2Layer, DebertaV2Model, DebertaV2Output, DebertaV2SelfOutput,
     DisentangledSelfAttention)
 
+from . import adapters as _adapters
 from . import relpos as _relpos
+from . import training as _training
 from ._cabi import host
 from .ops.flash_attention import _PENDING_STATUS, _check_pending, flash_attention_with_disentangled
 from .ops.flash_attention_varlen import flash_attention_with_disentangled_varlen
@@ -169,7 +171,8 @@ class FlashDisentangledSelfAttention(DisentangledSelfAttention):
         strided views, so no copy follows.  With gradients enabled, or a separate query input, the layers run as is."""
         H, D = self.num_attention_heads, self.attention_head_size
         lead = hidden_states.shape[:-1]
-        if query_states is hidden_states and not torch.is_grad_enabled():
+        if (query_states is hidden_states and not torch.is_grad_enabled()
+                and type(self.query_proj) is type(self.key_proj) is type(self.value_proj) is nn.Linear):
             qkv = torch.nn.functional.linear(hidden_states, *self._qkv_weights()).view(*lead, 3, H, D)
             return qkv.select(-3, 0), qkv.select(-3, 1), qkv.select(-3, 2)
         q = self.query_proj(query_states).view(*query_states.shape[:-1], H, D)
@@ -371,8 +374,8 @@ class FlashDebertaV2Encoder(DebertaV2Encoder):
             sa, so, act = att.self, att.output, layer.intermediate.intermediate_act_fn
             stock = (type(layer) in (DebertaV2Layer, FlashDebertaV2Layer)
                      and type(att) in (DebertaV2Attention, FlashDebertaV2Attention)
-                     and type(sa) is FlashDisentangledSelfAttention and type(so) is DebertaV2SelfOutput
-                     and type(up) is DebertaV2Intermediate and type(down) is DebertaV2Output
+                     and type(sa) is FlashDisentangledSelfAttention and type(so) in _training.SELF_OUTPUTS
+                     and type(up) is DebertaV2Intermediate and type(down) in _training.OUTPUTS
                      and (getattr(act, "act", None) is nn.functional.gelu
                           or (type(act) is nn.GELU and act.approximate == "none")))
             if not stock or sa.attention_head_size != 64:
@@ -383,11 +386,11 @@ class FlashDebertaV2Encoder(DebertaV2Encoder):
             norms = [so.LayerNorm, down.LayerNorm]
             if any(type(m) is not nn.Linear or m.bias is None for m in lins):
                 return None
-            if any(type(m) is not nn.LayerNorm or m.weight is None or m.bias is None for m in norms):
+            if any(type(m) not in _training.NORMS or m.weight is None or m.bias is None for m in norms):
                 return None
             drops = [so._modules.get("dropout"), down._modules.get("dropout")]
             drops += [sa._modules.get("pos_dropout")] if sa.relative_attention else []
-            if any(type(m) not in (nn.Dropout, nn.Identity) for m in drops):         # in eval mode both do nothing
+            if any(type(m) not in (*_training.DROPOUTS, nn.Identity) for m in drops):         # in eval mode both do nothing
                 return None
             hidden = so.dense.out_features
             widest = 1024 if so.dense.weight.dtype == torch.float32 else 2048
@@ -496,13 +499,14 @@ class FlashDebertaV2Encoder(DebertaV2Encoder):
         rel_embeddings = self.get_rel_embedding()
         all_hidden = (hidden_states,) if output_hidden_states else None
         n = len(self.layer)
-        for i, layer in enumerate(self.layer):
-            x, _ = layer(x, seqs, query_states=None, relative_pos=None, rel_embeddings=rel_embeddings,
-                         output_attentions=False)
-            if output_hidden_states:
-                last = i == n - 1
-                all_hidden = all_hidden + ((pad_input(x[0], indices, B, L) if (last or not self.skip_intermediate_padding)
-                                            else x),)
+        with _adapters.packed_rows(indices, B, L):
+            for i, layer in enumerate(self.layer):
+                x, _ = layer(x, seqs, query_states=None, relative_pos=None, rel_embeddings=rel_embeddings,
+                             output_attentions=False)
+                if output_hidden_states:
+                    last = i == n - 1
+                    all_hidden = all_hidden + ((pad_input(x[0], indices, B, L) if (last or not self.skip_intermediate_padding)
+                                                else x),)
         output_states = all_hidden[-1] if output_hidden_states else pad_input(x[0], indices, B, L)
         if not return_dict:
             return tuple(v for v in [output_states, all_hidden, None] if v is not None)
@@ -584,7 +588,7 @@ class FlashDebertaV2Model(DebertaV2Model):
         watch, of, plain = _PLANS.get(self, (None, None, None))
         if watch is None or of is not emb:
             if (type(emb) is not DebertaV2Embeddings or type(emb.word_embeddings) is not nn.Embedding
-                    or type(emb.LayerNorm) is not nn.LayerNorm or emb.word_embeddings.max_norm is not None
+                    or type(emb.LayerNorm) not in _training.NORMS or emb.word_embeddings.max_norm is not None
                     or any(getattr(emb, n, None) is not None for n in ("position_embeddings", "token_type_embeddings", "embed_proj"))):
                 return None
             watch = host.Watch(list(emb.modules()), [(emb.word_embeddings, ("max_norm",))])
@@ -626,9 +630,11 @@ class FlashDebertaV2Model(DebertaV2Model):
             _PASS.report = before
 
 
-def patch_model(model: nn.Module) -> nn.Module:
+def patch_model(model: nn.Module, train_kernels: bool = False) -> nn.Module:
     """Swap, in place, every eager ``DisentangledSelfAttention`` of an already built HF DeBERTa-v2 model for
-    the fused module (parameters are shared, not copied) and give its encoder the cached relative embeddings."""
+    the fused module (parameters are shared, not copied) and give its encoder the cached relative embeddings.
+    ``train_kernels``: passes that record gradients run their LayerNorms, dropouts and sublayer ends on this library's
+    kernels too (``training.py``); dropout then draws other numbers than torch's for the same seed."""
     for name, mod in list(model.named_modules()):
         if isinstance(mod, DebertaV2Attention) and not isinstance(mod.self, FlashDisentangledSelfAttention):
             old = mod.self
@@ -641,7 +647,7 @@ def patch_model(model: nn.Module) -> nn.Module:
             mod._rel_cache, mod._rel_cache_key, mod._rel_stamp = None, None, 0
         if type(mod) is DebertaV2Model:
             mod.__class__ = FlashDebertaV2Model
-    return model
+    return _training.use_train_kernels(model) if train_kernels else model
 
 
 class FlashDebertaV2ForMaskedLM(DebertaV2ForMaskedLM):
