@@ -11,9 +11,14 @@ struct Rows {
   explicit Rows(const Tensor& x) {
     cols = x.size(-1);
     rows = cols ? x.numel() / cols : 0;
+    stride = cols;
+    if (x.is_contiguous()) {                         // no view for what is read through its pointer anyway
+      t = x;
+      return;
+    }
     t = x.reshape({rows, cols});
     if (cols > 1 && t.stride(1) != 1) t = t.contiguous();
-    stride = rows > 1 ? t.stride(0) : cols;
+    if (rows > 1) stride = t.stride(0);
   }
   const void* ptr() const { return t.defined() ? t.data_ptr() : nullptr; }
 };
@@ -273,7 +278,8 @@ struct LoraCall {
   }
   Tensor floats(at::IntArrayRef sizes) const { return at::empty(sizes, w.options().dtype(at::kFloat)); }
   // The product alone, in fp32.
-  Tensor product(const Tensor& left, const Tensor& right) const {
+  Tensor product(const Tensor& rows, const Tensor& right) const {
+    const Tensor left = rows.dim() == 2 ? rows : rows.reshape({l.rows, rows.size(-1)});
     return l.dtype == TDB_DTYPE_F32 ? at::mm(left, right) : at::mm(left, right, at::kFloat);
   }
 };
@@ -295,6 +301,10 @@ Tensor lora_product(const LoraCall& c, bool back, const Tensor& f, const Tensor&
   const int64_t cols = back ? c.l.cols : c.l.features;
   if (c.tensor_cores) {
     Tensor y = at::empty({c.l.rows, cols}, c.w.options());
+    if (!back && tdb_lora_skinny_applies(&c.l)) {
+      check_rc(tdb_lora_skinny(&c.l, h.data_ptr(), y.data_ptr(), stream.stream()));
+      return y;
+    }
     StandingReport report(c.w.get_device(), stream);
     check_rc(tdb_lora_umma_product(&c.l, back, f.data_ptr(), h.data_ptr(), y.data_ptr(), report.words, stream.stream()));
     report.list();

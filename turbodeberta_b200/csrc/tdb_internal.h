@@ -216,4 +216,7 @@ TDB_HOST_API int tdb_lora_umma_gather(const tdb::Lora* l, int of_b, const void* 
 // a and b turned, either to null where it is not needed.
 TDB_HOST_API int tdb_lora_turn(const tdb::Lora* l, void* a_turned, void* b_turned, void* stream);
 TDB_HOST_API int tdb_lora_umma_gather_factors(const tdb::Lora* l);
+// `product` for a few rows (skinny.cu), forward only.
+TDB_HOST_API int tdb_lora_skinny_applies(const tdb::Lora* l);
+TDB_HOST_API int tdb_lora_skinny(const tdb::Lora* l, const void* hx, void* y, void* stream);
 }
