@@ -315,12 +315,20 @@ Tensor lora_product(const LoraCall& c, bool back, const Tensor& f, const Tensor&
   check_rc(tdb_lora_expand(&c.l, back, base.data_ptr<float>(), h.data_ptr<float>(), y.data_ptr(), stream.stream()));
   return y;
 }
-// y; the rows' inner values, from which the gradient of b is made; and, where the tensor cores will make gradients, which row is whose.
+// y; the rows' inner values, from which the gradient of b is made; and which row is whose, as the gradients' kernels want it.
 std::tuple<Tensor, Tensor, Tensor> run_lora(LoraCall& c, at::IntArrayRef shape, bool train) {
   const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream();
   if (c.l.rows == 0) return {at::empty(shape, c.w.options()), Tensor(), Tensor()};
   Tensor owners;
-  if (train && c.tensor_cores) owners = at::empty({(c.l.rows + 15) / 16, c.l.n}, c.w.options().dtype(at::kShort));
+  if (!c.tensor_cores) {
+    if (const int64_t words = tdb_lora_plan_words(&c.l)) {
+      owners = at::empty({words}, c.w.options().dtype(at::kInt));
+      check_rc(tdb_lora_plan(&c.l, owners.data_ptr<int32_t>(), stream.stream()));
+      c.l.plan = owners.data_ptr<int32_t>();
+    }
+  } else if (train) {
+    owners = at::empty({(c.l.rows + 15) / 16, c.l.n}, c.w.options().dtype(at::kShort));
+  }
   const Tensor h = lora_shrink(c, false, c.a, stream, owners);
   return {lora_product(c, false, c.b, h, stream).view(shape), h, owners};
 }
@@ -360,6 +368,7 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
     LoraCall c(x, w, std::nullopt, a, b, scaling.defined() ? OptTensor(scaling) : std::nullopt, ctx->saved_data["scaling"].toDouble(),
                ids.defined() ? OptTensor(ids) : std::nullopt);
     c.set_dy(grads[0]);
+    if (!c.tensor_cores && owners.defined()) c.l.plan = owners.data_ptr<int32_t>();
     Tensor dx, da, db, u;
     if (c.l.rows == 0) {
       if (need_x) dx = at::empty(x.sizes(), x.options());

@@ -11,7 +11,10 @@ struct LoraRows {
   int n;                                             // adapters
   const float* scaling;                              // one for each adapter; null: scaling_value
   float scaling_value;
+  // Rows sorted by adapter (lora.cu; null: as they come): position -> row, and each adapter's first position.  Ids are then those of positions.
+  const int32_t *order, *starts;
 };
+__device__ __forceinline__ int64_t row_at(const LoraRows& r, int64_t position) { return r.order ? r.order[position] : position; }
 __device__ __forceinline__ float scaling_of(const LoraRows& r, int adapter) { return r.scaling ? r.scaling[adapter] : r.scaling_value; }
 
 // -1 for a row without one: its id is not an adapter's.

@@ -774,7 +774,7 @@ __global__ void __launch_bounds__(256) turn_kernel(Turn first, Turn second) {
   }
 }
 
-LoraRows rows_of(const Lora& l) { return LoraRows{l.ids, l.id_bytes, l.rows_per_id, l.rows, l.n, l.scaling, l.scaling_value}; }
+LoraRows rows_of(const Lora& l) { return LoraRows{l.ids, l.id_bytes, l.rows_per_id, l.rows, l.n, l.scaling, l.scaling_value, nullptr, nullptr}; }
 int r16_of(const Lora& l) { return (l.rank + 15) / 16 * 16; }
 
 template <int MT, int NJ, int WARPS, int STAGES>

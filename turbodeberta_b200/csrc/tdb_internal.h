@@ -155,6 +155,7 @@ struct Lora {
   const void* ids;                                    // see LoraRows
   int id_bytes;
   int64_t rows_per_id;
+  const int32_t* plan;                                // of tdb_lora_plan(), or null; for the kernels of any type and size
 };
 }  // namespace tdb
 
@@ -196,7 +197,9 @@ TDB_HOST_API int tdb_norm_forward(const tdb::Norm* n, int dtype, void* stream);
 TDB_HOST_API int64_t tdb_norm_partial_floats(int64_t rows, int cols);
 TDB_HOST_API int tdb_norm_backward(const tdb::Norm* n, int dtype, void* stream);
 // Adapters beside a shared product, any type and size.  back: from dy through b and a instead of from x through a and b.  h: fp32 [rows, rank].
-// base: the product alone, fp32 [rows, columns of y].
+// base: the product alone, fp32 [rows, columns of y].  h lies in the order of l->plan, where there is one.
+TDB_HOST_API int64_t tdb_lora_plan_words(const tdb::Lora* l);
+TDB_HOST_API int tdb_lora_plan(const tdb::Lora* l, int32_t* plan, void* stream);
 TDB_HOST_API int tdb_lora_shrink(const tdb::Lora* l, int back, float* h, void* stream);
 TDB_HOST_API int tdb_lora_expand(const tdb::Lora* l, int back, const float* base, const float* h, void* y, void* stream);
 // The gradient of a (from v = u and x) or of b (from v = h and dy).  part: [shares, n, rank, columns] floats.  factors: of a block, 16 here.
