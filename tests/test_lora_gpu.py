@@ -82,7 +82,7 @@ def run(p, **more):
 
 SIZES = [(1, 64, 64, 8, 1), (1, 1024, 128, 16, 4), (2, 63, 65, 3, 2), (16, 1024, 256, 8, 16), (17, 128, 512, 64, 3), (33, 771, 773, 5, 3), (40, 8, 8, 1, 2),
          (64, 512, 320, 33, 5), (127, 72, 200, 16, 8), (129, 264, 128, 20, 4), (200, 1024, 1000, 16, 8), (300, 256, 264, 128, 2), (257, 640, 640, 100, 3),
-         (700, 200, 136, 4, 32), (513, 1, 3, 2, 2), (150, 128, 192, 256, 2)]
+         (700, 200, 136, 4, 32), (513, 1, 3, 2, 2), (150, 128, 192, 256, 2), (400, 64, 72, 2, 4095)]
 
 
 @pytest.mark.parametrize("dtype", [F, B])

@@ -285,11 +285,11 @@ struct LoraCall {
 };
 
 // The inner values of the rows: bf16 [rows, inner] from the tensor cores, else fp32 [rows, rank].  f: the factors, for the former.
-Tensor lora_shrink(const LoraCall& c, bool back, const Tensor& f, cudaStream_t stream, const Tensor& owners = {}) {
+Tensor lora_shrink(const LoraCall& c, bool back, const Tensor& f, cudaStream_t stream) {
   Tensor h;
   if (c.tensor_cores) {
     h = at::empty({c.l.rows, tdb_lora_inner(&c.l)}, c.w.options());
-    check_rc(tdb_lora_umma_shrink(&c.l, back, f.data_ptr(), h.data_ptr(), owners.defined() ? static_cast<uint16_t*>(owners.data_ptr()) : nullptr, stream));
+    check_rc(tdb_lora_umma_shrink(&c.l, back, f.data_ptr(), h.data_ptr(), stream));
   } else {
     h = c.floats({c.l.rows, c.l.rank});
     check_rc(tdb_lora_shrink(&c.l, back, h.data_ptr<float>(), stream));
@@ -315,30 +315,27 @@ Tensor lora_product(const LoraCall& c, bool back, const Tensor& f, const Tensor&
   check_rc(tdb_lora_expand(&c.l, back, base.data_ptr<float>(), h.data_ptr<float>(), y.data_ptr(), stream.stream()));
   return y;
 }
-// y; the rows' inner values, from which the gradient of b is made; and which row is whose, as the gradients' kernels want it.
+// y; the rows' inner values, from which the gradient of b is made; and the rows' order by adapter, where the kernels go by it.
 std::tuple<Tensor, Tensor, Tensor> run_lora(LoraCall& c, at::IntArrayRef shape, bool train) {
   const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream();
   if (c.l.rows == 0) return {at::empty(shape, c.w.options()), Tensor(), Tensor()};
-  Tensor owners;
-  if (!c.tensor_cores) {
-    if (const int64_t words = tdb_lora_plan_words(&c.l)) {
-      owners = at::empty({words}, c.w.options().dtype(at::kInt));
-      check_rc(tdb_lora_plan(&c.l, owners.data_ptr<int32_t>(), stream.stream()));
-      c.l.plan = owners.data_ptr<int32_t>();
-    }
-  } else if (train) {
-    owners = at::empty({(c.l.rows + 15) / 16, c.l.n}, c.w.options().dtype(at::kShort));
+  Tensor plan;
+  const int64_t words = c.tensor_cores && !train ? 0 : tdb_lora_plan_words(&c.l, c.tensor_cores);
+  if (words) {
+    plan = at::empty({words}, c.w.options().dtype(at::kInt));
+    check_rc(tdb_lora_plan(&c.l, plan.data_ptr<int32_t>(), stream.stream()));
+    c.l.plan = plan.data_ptr<int32_t>();
   }
-  const Tensor h = lora_shrink(c, false, c.a, stream, owners);
-  return {lora_product(c, false, c.b, h, stream).view(shape), h, owners};
+  const Tensor h = lora_shrink(c, false, c.a, stream);
+  return {lora_product(c, false, c.b, h, stream).view(shape), h, plan};
 }
 
-Tensor lora_gradient(const LoraCall& c, bool of_b, const Tensor& v, const Tensor& owners, cudaStream_t stream) {
+Tensor lora_gradient(const LoraCall& c, bool of_b, const Tensor& v, cudaStream_t stream) {
   const Tensor& like = of_b ? c.b : c.a;
   if (c.l.rows == 0) return at::zeros_like(like);
   const int shares = tdb_lora_gather_shares(&c.l, of_b, c.tensor_cores ? tdb_lora_umma_gather_factors(&c.l) : 16);
   Tensor part = c.floats({shares, c.l.n, c.l.rank, of_b ? c.l.features : c.l.cols}), out = at::empty(like.sizes(), like.options());
-  if (c.tensor_cores) check_rc(tdb_lora_umma_gather(&c.l, of_b, v.data_ptr(), static_cast<const uint16_t*>(owners.data_ptr()), part.data_ptr<float>(), shares, stream));
+  if (c.tensor_cores) check_rc(tdb_lora_umma_gather(&c.l, of_b, v.data_ptr(), part.data_ptr<float>(), shares, stream));
   else check_rc(tdb_lora_gather(&c.l, of_b, v.data_ptr<float>(), part.data_ptr<float>(), shares, stream));
   check_rc(tdb_lora_gather_sum(&c.l, of_b, part.data_ptr<float>(), shares, out.data_ptr(), stream));
   return out;
@@ -351,8 +348,8 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
     at::AutoDispatchBelowAutograd below;
     c10::cuda::CUDAGuard guard(x.device());
     LoraCall c(x, w, bias, a, b, scaling, scaling_value, ids);
-    auto [y, h, owners] = run_lora(c, shape, a.requires_grad() || b.requires_grad());
-    ctx->save_for_backward({x, w, a, b, scaling ? *scaling : Tensor(), ids ? *ids : Tensor(), b.requires_grad() ? h : Tensor(), owners});
+    auto [y, h, plan] = run_lora(c, shape, a.requires_grad() || b.requires_grad());
+    ctx->save_for_backward({x, w, a, b, scaling ? *scaling : Tensor(), ids ? *ids : Tensor(), b.requires_grad() ? h : Tensor(), plan});
     ctx->saved_data["scaling"] = scaling_value;
     ctx->saved_data["bias"] = bias.has_value();
     return y;
@@ -360,7 +357,7 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     refuse_second_derivative("lora_linear");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &a = saved[2], &b = saved[3], &scaling = saved[4], &ids = saved[5], &h = saved[6], &owners = saved[7];
+    const Tensor &x = saved[0], &w = saved[1], &a = saved[2], &b = saved[3], &scaling = saved[4], &ids = saved[5], &h = saved[6], &plan = saved[7];
     const int at = ctx->saved_data["bias"].toBool() ? 3 : 2;
     const bool need_x = ctx->needs_input_grad(0), need_a = ctx->needs_input_grad(at), need_b = ctx->needs_input_grad(at + 1);
     c10::cuda::CUDAGuard guard(x.device());
@@ -368,7 +365,7 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
     LoraCall c(x, w, std::nullopt, a, b, scaling.defined() ? OptTensor(scaling) : std::nullopt, ctx->saved_data["scaling"].toDouble(),
                ids.defined() ? OptTensor(ids) : std::nullopt);
     c.set_dy(grads[0]);
-    if (!c.tensor_cores && owners.defined()) c.l.plan = owners.data_ptr<int32_t>();
+    if (plan.defined()) c.l.plan = plan.data_ptr<int32_t>();
     Tensor dx, da, db, u;
     if (c.l.rows == 0) {
       if (need_x) dx = at::empty(x.sizes(), x.options());
@@ -383,8 +380,8 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
       u = lora_shrink(c, true, b_turned, stream);
       if (need_x) dx = lora_product(c, true, a_turned, u, stream).view(x.sizes());
     }
-    if (need_a) da = lora_gradient(c, false, u, owners, stream);
-    if (need_b) db = lora_gradient(c, true, h, owners, stream);
+    if (need_a) da = lora_gradient(c, false, u, stream);
+    if (need_b) db = lora_gradient(c, true, h, stream);
     const Tensor none;
     return {dx, none, none, da, db, none, none, none, none};
   }

@@ -42,13 +42,14 @@ __device__ __forceinline__ void find_present(Present& s, const LoraRows& rows, i
 // Positions of the rows in the order of their adapters, rows without one last, each adapter's in their own order (the sums of gradients then have
 // a fixed order too).  One block: every warp counts its share of the rows by adapter, the counts are added up adapter by adapter, and the
 // warps go through their rows once more.  plan: [bins + 1] first positions, [rows] rows, [rows] ids; bins = n + 1.
-constexpr int SORT_WARPS = 32, SORT_MOST = 1023;
-__global__ void __launch_bounds__(SORT_WARPS * 32) sort_kernel(LoraRows rows, int32_t* __restrict__ plan) {
+constexpr int SORT_BYTES = 200 * 1024;
+int sort_warps(int n) { return std::min(32, SORT_BYTES / 4 / (n + 1)); }
+__global__ void __launch_bounds__(1024) sort_kernel(LoraRows rows, int32_t* __restrict__ plan) {
   extern __shared__ int counts[];                    // [warps][bins]
-  __shared__ int sums[SORT_WARPS];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, bins = rows.n + 1;
+  __shared__ int sums[32];
+  const int warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32, bins = rows.n + 1;
   int* mine = counts + warp * bins;
-  const int64_t share = (rows.rows + SORT_WARPS * 32 - 1) / (SORT_WARPS * 32) * 32, begin = warp * share, end = min(rows.rows, begin + share);
+  const int64_t share = (rows.rows + blockDim.x - 1) / blockDim.x * 32, begin = warp * share, end = min(rows.rows, begin + share);
   int32_t *order = plan + bins + 1, *ids = order + rows.rows;
   for (int i = lane; i < bins; i += 32) mine[i] = 0;
   __syncwarp();
@@ -65,10 +66,11 @@ __global__ void __launch_bounds__(SORT_WARPS * 32) sort_kernel(LoraRows rows, in
   };
   walk([](int64_t, int, int, int) {});
   __syncthreads();
-  // exclusive sums, adapter by adapter and within one warp by warp; a thread has one bin
+  // exclusive sums, adapter by adapter and within one warp by warp; a thread has neighbouring bins
+  const int each = (bins + blockDim.x - 1) / blockDim.x, first = threadIdx.x * each, last = min(bins, first + each);
   int total = 0;
-  if ((int)threadIdx.x < bins)
-    for (int w = 0; w < SORT_WARPS; ++w) total += counts[w * bins + threadIdx.x];
+  for (int i = first; i < last; ++i)
+    for (int w = 0; w < warps; ++w) total += counts[w * bins + i];
   int run = total;
 #pragma unroll
   for (int off = 1; off < 32; off *= 2) {
@@ -79,15 +81,15 @@ __global__ void __launch_bounds__(SORT_WARPS * 32) sort_kernel(LoraRows rows, in
   __syncthreads();
   int base = run - total;
   for (int w = 0; w < warp; ++w) base += sums[w];
-  if ((int)threadIdx.x < bins) {
-    plan[threadIdx.x] = base;
-    if ((int)threadIdx.x == bins - 1) plan[bins] = base + total;
-    for (int w = 0; w < SORT_WARPS; ++w) {
-      const int n = counts[w * bins + threadIdx.x];
-      counts[w * bins + threadIdx.x] = base;
+  for (int i = first; i < last; ++i) {
+    plan[i] = base;
+    for (int w = 0; w < warps; ++w) {
+      const int n = counts[w * bins + i];
+      counts[w * bins + i] = base;
       base += n;
     }
   }
+  if (threadIdx.x == 0) plan[bins] = (int)rows.rows;
   __syncthreads();
   walk([&](int64_t row, int id, int bin, int rank) {
     const int at = mine[bin] + rank;
@@ -96,10 +98,10 @@ __global__ void __launch_bounds__(SORT_WARPS * 32) sort_kernel(LoraRows rows, in
   });
 }
 
-// h[t][j] = s_a sum over the columns of x[t][c] F_a(j, c).  A block: four rows; its warps share the columns, eight factors at a time, so that a
-// thread's 12 loads feed 32 products.  Bound by the factors' way through the first-level cache.
-constexpr int S_ROWS = 4, S_WARPS = 8, S_FACTORS = 8;
-template <typename T>
+// h[t][j] = s_a sum over the columns of x[t][c] F_a(j, c).  A block: S_ROWS rows (four, or eight where there are enough of them); its warps share the
+// columns, eight factors at a time, so that a thread's 16 loads feed 64 products.  Bound by the factors' way through the caches.
+constexpr int S_WARPS = 8, S_FACTORS = 8;
+template <typename T, int S_ROWS>
 __global__ void __launch_bounds__(S_WARPS * 32) shrink_kernel(const T* __restrict__ x, int64_t stride, int cols, Factors<T> f, int rank, LoraRows rows,
                                                              float* __restrict__ h) {
   __shared__ Present here;
@@ -131,23 +133,26 @@ __global__ void __launch_bounds__(S_WARPS * 32) shrink_kernel(const T* __restric
         for (int j = 0; j < S_FACTORS; ++j) acc[r][j] = fmaf(xv[r], fv[j], acc[r][j]);
     }
     // 32 sums over 32 lanes: lanes trade halves, and lane l ends with sum l
-    float v[32];
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = acc[i / S_FACTORS][i % S_FACTORS];
+    for (int k0 = 0; k0 < S_ROWS; k0 += 4) {
+      float v[32];
 #pragma unroll
-    for (int half = 16; half >= 1; half >>= 1) {
-      const bool up = lane & half;
+      for (int i = 0; i < 32; ++i) v[i] = acc[k0 + i / S_FACTORS][i % S_FACTORS];
 #pragma unroll
-      for (int i = 0; i < half; ++i) v[i] = (up ? v[i + half] : v[i]) + __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + half], half);
+      for (int half = 16; half >= 1; half >>= 1) {
+        const bool up = lane & half;
+#pragma unroll
+        for (int i = 0; i < half; ++i) v[i] = (up ? v[i + half] : v[i]) + __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + half], half);
+      }
+      part[warp][k0 * S_FACTORS + lane] = v[0];
     }
     __syncthreads();
-    part[warp][lane] = v[0];
-    __syncthreads();
-    if (warp == 0) {
+    if (threadIdx.x < S_ROWS * S_FACTORS) {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < S_WARPS; ++w) s += part[w][lane];
-      const int r = lane / S_FACTORS, j = j0 + lane % S_FACTORS;
+      for (int w = 0; w < S_WARPS; ++w) s += part[w][threadIdx.x];
+      const int r = threadIdx.x / S_FACTORS, j = j0 + threadIdx.x % S_FACTORS;
       if (here.id[r] == a && j < rank) h[(t0 + r) * rank + j] = s * scaling_of(rows, a);
     }
   }
@@ -158,7 +163,7 @@ template <typename T>
 __global__ void __launch_bounds__(COLS) expand_kernel(const float* base, const T* __restrict__ bias, const float* __restrict__ h, int rank, Factors<T> f,
                                                       LoraRows rows, int cols, T* y) {     // base may be y
   __shared__ Present here;
-  __shared__ float hs[TILE][64];
+  __shared__ __align__(16) float hs[TILE][64];
   const int64_t t0 = (int64_t)blockIdx.x * TILE;
   const int c = blockIdx.y * COLS + threadIdx.x;
   __shared__ int64_t place[TILE];
@@ -182,14 +187,38 @@ __global__ void __launch_bounds__(COLS) expand_kernel(const float* base, const T
     for (int k = 0; k < here.count; ++k) {
       const int a = here.list[k];
       const T* fa = f.p + a * f.each + j0 * f.sj + (int64_t)c * f.sc;
-      uint32_t mine = 0;
+      uint32_t mine = 0, absent = 0;
 #pragma unroll
-      for (int r = 0; r < TILE; ++r) mine |= (here.id[r] == a ? 1u : 0u) << r;
-#pragma unroll 4
-      for (int j = 0; j < jn; ++j) {
-        const float v = value(fa + j * f.sj);
+      for (int r = 0; r < TILE; ++r) {
+        mine |= (here.id[r] == a ? 1u : 0u) << r;
+        absent |= (t0 + r >= rows.rows ? 1u : 0u) << r;
+      }
+      const bool vectors = sizeof(T) == 4 && f.sj == 1 && rank % 4 == 0 && (reinterpret_cast<uintptr_t>(fa) & 15) == 0;
+      const bool whole = (mine | absent) == (1u << TILE) - 1u;
+#pragma unroll 2
+      for (int j = 0; j < jn; j += 4) {
+        float v[4];
+        if (vectors) {
+          const float4 q = *reinterpret_cast<const float4*>(fa + j);
+          v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+        } else {
 #pragma unroll
-        for (int r = 0; r < TILE; ++r) acc[r] = mine >> r & 1 ? fmaf(hs[r][j], v, acc[r]) : acc[r];
+          for (int i = 0; i < 4; ++i) v[i] = j + i < jn ? value(fa + (j + i) * f.sj) : 0.f;
+        }
+        if (whole) {
+#pragma unroll
+          for (int r = 0; r < TILE; ++r) {
+            const float4 q = *reinterpret_cast<const float4*>(&hs[r][j]);
+            acc[r] = fmaf(q.w, v[3], fmaf(q.z, v[2], fmaf(q.y, v[1], fmaf(q.x, v[0], acc[r]))));
+          }
+        } else {                                     // other rows' zeros must not meet what may not be finite
+#pragma unroll
+          for (int r = 0; r < TILE; ++r) {
+            const float4 q = *reinterpret_cast<const float4*>(&hs[r][j]);
+            const float s = fmaf(q.w, v[3], fmaf(q.z, v[2], fmaf(q.y, v[1], fmaf(q.x, v[0], acc[r]))));
+            acc[r] = mine >> r & 1 ? s : acc[r];
+          }
+        }
       }
     }
   }
@@ -206,7 +235,7 @@ __global__ void __launch_bounds__(COLS) gather_kernel(const T* __restrict__ x, i
                                                       LoraRows rows, int j_blocks, float* __restrict__ part) {
   __shared__ int ids[32];
   __shared__ int64_t place[32];
-  __shared__ float vs[32][16];
+  __shared__ __align__(16) float vs[32][16];
   const int a = blockIdx.y / j_blocks, j0 = blockIdx.y % j_blocks * 16, jn = min(16, rank - j0), c = blockIdx.x * COLS + threadIdx.x;
   // sorted rows: a share of the adapter's own positions, otherwise of all
   const int64_t first = rows.starts ? rows.starts[a] : 0, last = rows.starts ? rows.starts[a + 1] : rows.rows;
@@ -272,18 +301,15 @@ __global__ void __launch_bounds__(256) gather_sum_turned_kernel(const float* __r
   if (j0 + j < rank && c0 + c < cols) put(out + (a * cols + c0 + c) * rank + j0 + j, s[j][c]);
 }
 
-LoraRows rows_of(const Lora& l) {
-  if (!l.plan) return LoraRows{l.ids, l.id_bytes, l.rows_per_id, l.rows, l.n, l.scaling, l.scaling_value, nullptr, nullptr};
-  const int32_t* order = l.plan + l.n + 2;
-  return LoraRows{order + l.rows, 4, 1, l.rows, l.n, l.scaling, l.scaling_value, order, l.plan};
-}
-
 template <typename T>
 int shrink(const Lora& l, bool back, float* h, cudaStream_t s) {
   const int cols = back ? l.features : l.cols;
   const Factors<T> f = back ? Factors<T>{(const T*)l.b, (int64_t)l.features * l.rank, 1, l.rank} : Factors<T>{(const T*)l.a, (int64_t)l.cols * l.rank, l.cols, 1};
-  const dim3 grid((unsigned)((l.rows + S_ROWS - 1) / S_ROWS), (l.rank + S_FACTORS - 1) / S_FACTORS);
-  shrink_kernel<T><<<grid, S_WARPS * 32, 0, s>>>((const T*)(back ? l.dy : l.x), back ? l.dy_stride : l.x_stride, cols, f, l.rank, rows_of(l), h);
+  int sms = 0;
+  if (const int rc = device_sms(&sms)) return rc;
+  const int js = (l.rank + S_FACTORS - 1) / S_FACTORS, each = (l.rows + 7) / 8 * js >= sms ? 8 : 4;
+  const dim3 grid((unsigned)((l.rows + each - 1) / each), js);
+  (each == 8 ? shrink_kernel<T, 8> : shrink_kernel<T, 4>)<<<grid, S_WARPS * 32, 0, s>>>((const T*)(back ? l.dy : l.x), back ? l.dy_stride : l.x_stride, cols, f, l.rank, lora_rows(l), h);
   return cuda_fail(cudaGetLastError(), "lora shrink launch");
 }
 template <typename T>
@@ -291,14 +317,14 @@ int expand(const Lora& l, bool back, const float* base, const float* h, void* y,
   const int cols = back ? l.cols : l.features;
   const Factors<T> f = back ? Factors<T>{(const T*)l.a, (int64_t)l.cols * l.rank, l.cols, 1} : Factors<T>{(const T*)l.b, (int64_t)l.features * l.rank, 1, l.rank};
   const dim3 grid((unsigned)((l.rows + TILE - 1) / TILE), (cols + COLS - 1) / COLS);
-  expand_kernel<T><<<grid, COLS, 0, s>>>(base, back ? nullptr : (const T*)l.bias, h, l.rank, f, rows_of(l), cols, (T*)y);
+  expand_kernel<T><<<grid, COLS, 0, s>>>(base, back ? nullptr : (const T*)l.bias, h, l.rank, f, lora_rows(l), cols, (T*)y);
   return cuda_fail(cudaGetLastError(), "lora expand launch");
 }
 template <typename T>
 int gather(const Lora& l, bool of_b, const float* v, float* part, int shares, cudaStream_t s) {
   const int cols = of_b ? l.features : l.cols, j_blocks = (l.rank + 15) / 16;
   const dim3 grid((cols + COLS - 1) / COLS, l.n * j_blocks, shares);
-  gather_kernel<T><<<grid, COLS, 0, s>>>((const T*)(of_b ? l.dy : l.x), of_b ? l.dy_stride : l.x_stride, cols, v, l.rank, rows_of(l), j_blocks, part);
+  gather_kernel<T><<<grid, COLS, 0, s>>>((const T*)(of_b ? l.dy : l.x), of_b ? l.dy_stride : l.x_stride, cols, v, l.rank, lora_rows(l), j_blocks, part);
   return cuda_fail(cudaGetLastError(), "lora gather launch");
 }
 template <typename T>
@@ -317,18 +343,20 @@ using namespace tdb;
 
 extern "C" {
 
-// Words of the plan that puts the rows in their adapters' order, 0 where it does not pay: a single adapter, few rows (a training step of 700
-// rows in long requests of three adapters, fp32: 124 us without, 128 with), or more adapters than the block can count.
-int64_t tdb_lora_plan_words(const Lora* l) {
-  return l->n > 1 && l->n <= SORT_MOST && l->rows >= 256 && l->rows < (int64_t)1 << 30 ? l->n + 2 + 2 * l->rows : 0;
+// Words of the plan that puts the rows in their adapters' order, 0 where there is none.  The tensor cores' gradients want it (`train`) wherever rows have
+// ids; the other kernels from 256 rows and two adapters on (a training step of 700 rows in long requests of three adapters, fp32: 124 us without,
+// 128 with).
+int64_t tdb_lora_plan_words(const Lora* l, int train) {
+  const bool wanted = train ? l->ids != nullptr : l->n > 1 && l->rows >= 256;
+  return wanted && l->rows < (int64_t)1 << 30 ? l->n + 2 + 2 * l->rows : 0;
 }
 int tdb_lora_plan(const Lora* l, int32_t* plan, void* stream) {
-  const int smem = SORT_WARPS * (l->n + 1) * 4;
+  const int warps = sort_warps(l->n), smem = warps * (l->n + 1) * 4;
   if (smem > 48 * 1024)
-    if (const int rc = opt_in_smem(reinterpret_cast<const void*>(sort_kernel), SORT_WARPS * (SORT_MOST + 1) * 4)) return rc;
+    if (const int rc = opt_in_smem(reinterpret_cast<const void*>(sort_kernel), SORT_BYTES)) return rc;
   Lora plain = *l;
   plain.plan = nullptr;
-  sort_kernel<<<1, SORT_WARPS * 32, smem, (cudaStream_t)stream>>>(rows_of(plain), plan);
+  sort_kernel<<<1, warps * 32, smem, (cudaStream_t)stream>>>(lora_rows(plain), plan);
   return cuda_fail(cudaGetLastError(), "lora sort launch");
 }
 

@@ -25,4 +25,16 @@ __device__ __forceinline__ int adapter_of(const LoraRows& r, int64_t row) {
   return id >= 0 && id < r.n ? (int)id : -1;
 }
 
+// Of a call, in the order of its plan where it has one.
+inline LoraRows lora_rows(const Lora& l) {
+  if (!l.plan) return LoraRows{l.ids, l.id_bytes, l.rows_per_id, l.rows, l.n, l.scaling, l.scaling_value, nullptr, nullptr};
+  const int32_t* order = l.plan + l.n + 2;
+  return LoraRows{order + l.rows, 4, 1, l.rows, l.n, l.scaling, l.scaling_value, order, l.plan};
+}
+inline LoraRows lora_rows_as_they_come(const Lora& l) {
+  Lora plain = l;
+  plain.plan = nullptr;
+  return lora_rows(plain);
+}
+
 }  // namespace tdb

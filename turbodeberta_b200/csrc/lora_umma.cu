@@ -75,33 +75,28 @@ struct Adapters {
 // hx[t] = the inner values of row t: r16 high parts, r16 low parts.  A block: 16 MT rows and 8 NJ factors; its warps share the columns, blocks of
 // 64 in turn, and add up through shared memory.  Bound by reading x, and the factors from L2 once for every block: each warp has STAGES blocks
 // of columns on their way into shared memory that is its own, so that nothing waits for the block's other warps.
-// blockIdx.z takes every gridDim.z-th adapter of the rows.  owners [rows / 16][n], where it is wanted: for the gradients, which of the rows are whose.
+// blockIdx.z takes every gridDim.z-th adapter of the rows.  Rows may come sorted by adapter (lora.cu); what is read and written then is the row at each position.
 template <int MT, int NJ> __host__ __device__ constexpr int shrink_stage() { return (16 * MT + 8 * NJ) * 128; }
 
 template <int MT, int NJ, int WARPS, int STAGES>
 __global__ void __launch_bounds__(WARPS * 32) shrink_mma_kernel(const bf16* __restrict__ x, int64_t stride, int cols, const bf16* __restrict__ f, int rank,
-                                                                int r16, LoraRows rows, bf16* __restrict__ hx, uint16_t* __restrict__ owners) {
+                                                                int r16, LoraRows rows, bf16* __restrict__ hx) {
   extern __shared__ __align__(128) uint8_t ring[];     // [warps][stages][rows of x, then factors][64]; then the warps' sums
-  __shared__ int ids[16 * MT];
+  __shared__ int ids[16 * MT], place[16 * MT];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4, j0 = blockIdx.y * 8 * NJ;
   const int64_t t0 = (int64_t)blockIdx.x * 16 * MT;
   let_next_start();
-  if (threadIdx.x < 16 * MT) ids[threadIdx.x] = t0 + threadIdx.x < rows.rows ? adapter_of(rows, t0 + threadIdx.x) : -1;
+  if (threadIdx.x < 16 * MT) {
+    const bool in = t0 + threadIdx.x < rows.rows;
+    ids[threadIdx.x] = in ? adapter_of(rows, t0 + threadIdx.x) : -1;
+    place[threadIdx.x] = in ? (int)row_at(rows, t0 + threadIdx.x) : 0;
+  }
   __syncthreads();
   constexpr int N = (16 * MT + 31) / 32, STAGE = shrink_stage<MT, NJ>();
   Adapters<N> adapters;
 #pragma unroll
   for (int i = 0; i < N; ++i) { adapters.id[i] = 32 * i + lane < 16 * MT ? ids[32 * i + lane] : -1; adapters.high[i] = 0; }
   adapters.start(rows.n);
-  if (owners && blockIdx.y == 0 && blockIdx.z == 0)    // which of sixteen rows are an adapter's, for every adapter
-    for (int e = threadIdx.x; e < MT * rows.n; e += WARPS * 32) {
-      const int m = e / rows.n, a = e % rows.n;
-      if (t0 + 16 * m >= rows.rows) break;
-      uint32_t mask = 0;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mask |= (ids[16 * m + r] == a ? 1u : 0u) << r;
-      owners[((t0 >> 4) + m) * rows.n + a] = (uint16_t)mask;
-    }
   const uint32_t mine = smem_u32(ring) + warp * STAGES * STAGE;
   const int blocks = (cols + 63) / 64, n = blocks > warp ? (blocks - warp + WARPS - 1) / WARPS : 0;      // blocks of columns, and this warp's of them
   float* part = reinterpret_cast<float*>(ring);        // [warps][16 MT][8 NJ]
@@ -119,7 +114,7 @@ __global__ void __launch_bounds__(WARPS * 32) shrink_mma_kernel(const bf16* __re
           const int r = 4 * k + lane / 8;
           const bool of_x = r < 16 * MT;
           const bool in = c < cols && (of_x ? t0 + r < rows.rows : j0 + r - 16 * MT < rank);
-          const bf16* src = of_x ? x + (t0 + r) * stride + c : fa + (int64_t)(r - 16 * MT) * cols + c;
+          const bf16* src = of_x ? x + place[r] * stride + c : fa + (int64_t)(r - 16 * MT) * cols + c;
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + r * 128 + ((lane % 8 ^ (r & 7)) << 4)), "l"(in ? src : x), "r"(in ? 16 : 0) : "memory");
         }
       }
@@ -178,7 +173,7 @@ __global__ void __launch_bounds__(WARPS * 32) shrink_mma_kernel(const bf16* __re
       s *= scale;
       const bf16 high = __float2bfloat16_rn(s);
       const float rest = s - __bfloat162float(high);
-      bf16* out = hx + (t0 + row) * 2 * r16 + j0 + j;
+      bf16* out = hx + (int64_t)place[row] * 2 * r16 + j0 + j;
       out[0] = high;
       out[r16] = __float2bfloat16_rn(isfinite(rest) ? rest : 0.f);
     }
@@ -640,24 +635,24 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
 
 // ------------------------------------------------------------------------------------------------------------------- gather
 // part[z][a][j][c] = sum over a share of the rows t of adapter a of v[t][j] x[t][c], v being the sum of two bf16 numbers.  A block: one
-// adapter, 16 MT factors, 128 columns; a warp: 16 columns.  Rows come in tiles of 64 through shared memory, two at a time; tiles without
-// a row of the adapter are passed over, and other rows of a tile are zeros in both operands.  Of the tiles with one, blockIdx.z takes every
-// gridDim.z-th: ranges of rows would leave most blocks without work where requests are long (8192 rows, four adapters: 46 us).  Bound by reading x.
-constexpr int GC = 128, GP = GC + 8, G_BATCH = 256;
+// adapter, 16 MT factors, 128 columns; a warp: 16 columns.  The adapter's rows, which the plan lists, come in tiles of 64 through shared memory, two at
+// a time; blockIdx.z takes every gridDim.z-th tile.  Bound by reading x.
+constexpr int GC = 128, GP = GC + 8, G_BATCH = 16;     // G_BATCH: tiles whose rows are looked up at once
 __host__ __device__ constexpr int gather_pitch(int mt) { return 32 * mt + 8; }
 __host__ __device__ constexpr int gather_smem(int mt) { return 2 * 64 * (GP + gather_pitch(mt)) * 2; }
 
 template <int MT>
 __global__ void __launch_bounds__(256) gather_mma_kernel(const bf16* __restrict__ x, int64_t stride, int cols, const bf16* __restrict__ v, int r16, int rank,
-                                                         const uint16_t* __restrict__ owners, int64_t rows, int n_adapters, int j_blocks, float* __restrict__ part) {
+                                                         const int32_t* __restrict__ order, const int32_t* __restrict__ starts, int rows, int n_adapters, int j_blocks,
+                                                         float* __restrict__ part) {
   constexpr int VP = gather_pitch(MT);
   extern __shared__ __align__(16) bf16 tiles[];
-  __shared__ uint64_t masks[G_BATCH];
-  __shared__ int list[G_BATCH], listed;
+  __shared__ int place[G_BATCH * 64];                  // -1: behind the adapter's last row
   bf16 *xs[2] = {tiles, tiles + 64 * GP}, *vs[2] = {tiles + 2 * 64 * GP, tiles + 2 * 64 * GP + 64 * VP};
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int a = blockIdx.y / j_blocks, j0 = blockIdx.y % j_blocks * 16 * MT, c0 = blockIdx.x * GC;
-  uint32_t seen = 0;                                   // tiles with a row of the adapter so far
+  const int first = starts ? starts[a] : 0, last = starts ? starts[a + 1] : rows, all = (last - first + 63) / 64;
+  const int mine = all > (int)blockIdx.z ? (all - blockIdx.z + gridDim.z - 1) / gridDim.z : 0;       // tiles of this block
   float acc[MT][2][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -669,53 +664,33 @@ __global__ void __launch_bounds__(256) gather_mma_kernel(const bf16* __restrict_
   auto copy = [](bf16* dst, const bf16* src, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(saddr(dst)), "l"(src), "r"(real ? 16 : 0) : "memory");
   };
-  for (int64_t batch = 0; batch < rows; batch += 64 * G_BATCH) {
-    const int n = (int)min((int64_t)G_BATCH, (rows - batch + 63) / 64);
+  for (int batch = 0; batch < mine; batch += G_BATCH) {
+    const int todo = min(G_BATCH, mine - batch);
     __syncthreads();
-    if (tid < n) {
-      uint64_t m = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (batch + 64 * tid + 16 * i < rows) m |= (uint64_t)owners[((batch >> 4) + 4 * tid + i) * n_adapters + a] << (16 * i);
-      masks[tid] = m;
+    for (int e = tid; e < todo * 64; e += 256) {
+      const int at = first + ((batch + e / 64) * gridDim.z + blockIdx.z) * 64 + e % 64;
+      place[e] = at >= last ? -1 : order ? order[at] : at;
     }
     __syncthreads();
-    if (warp == 0) {
-      int mine = 0;
-      for (int i0 = 0; i0 < n; i0 += 32) {
-        const bool any = i0 + lane < n && masks[i0 + lane] != 0;
-        const uint32_t with = __ballot_sync(0xffffffffu, any), before = (1u << lane) - 1u;
-        const bool ours = any && (seen + __popc(with & before)) % gridDim.z == blockIdx.z;
-        const uint32_t all = __ballot_sync(0xffffffffu, ours);
-        if (ours) list[mine + __popc(all & before)] = i0 + lane;
-        mine += __popc(all);
-        seen += __popc(with);
-      }
-      if (lane == 0) listed = mine;
-    }
-    __syncthreads();
-    const int todo = listed;
     auto load = [&](int i, int buf) {
-      const uint64_t m = masks[i];
-      const int64_t t0 = batch + 64 * i;
 #pragma unroll
       for (int k = 0; k < 64 * GC / 8 / 256; ++k) {
-        const int e = tid + 256 * k, r = e / (GC / 8), c = e % (GC / 8) * 8;
-        const bool real = m >> r & 1 && c0 + c < cols;
-        copy(xs[buf] + r * GP + c, x + (real ? (t0 + r) * stride + c0 + c : 0), real);
+        const int e = tid + 256 * k, r = e / (GC / 8), c = e % (GC / 8) * 8, row = place[i * 64 + r];
+        const bool real = row >= 0 && c0 + c < cols;
+        copy(xs[buf] + r * GP + c, x + (real ? row * stride + c0 + c : 0), real);
       }
 #pragma unroll
       for (int k = 0; k < 64 * 4 * MT / 256; ++k) {    // 2 MT pieces of high parts, 2 MT of low ones
-        const int e = tid + 256 * k, r = e / (4 * MT), q = e % (4 * MT), low = q / (2 * MT), j = j0 + q % (2 * MT) * 8;
-        const bool real = m >> r & 1 && j < r16;
-        copy(vs[buf] + r * VP + q * 8, v + (real ? (t0 + r) * 2 * r16 + low * r16 + j : 0), real);
+        const int e = tid + 256 * k, r = e / (4 * MT), q = e % (4 * MT), low = q / (2 * MT), j = j0 + q % (2 * MT) * 8, row = place[i * 64 + r];
+        const bool real = row >= 0 && j < r16;
+        copy(vs[buf] + r * VP + q * 8, v + (real ? (int64_t)row * 2 * r16 + low * r16 + j : 0), real);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (todo > 0) load(list[0], 0);
+    load(0, 0);
     for (int i = 0, buf = 0; i < todo; ++i, buf ^= 1) {
       if (i + 1 < todo) {
-        load(list[i + 1], buf ^ 1);
+        load(i + 1, buf ^ 1);
         asm volatile("cp.async.wait_group 1;" ::: "memory");
       } else {
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -774,11 +749,10 @@ __global__ void __launch_bounds__(256) turn_kernel(Turn first, Turn second) {
   }
 }
 
-LoraRows rows_of(const Lora& l) { return LoraRows{l.ids, l.id_bytes, l.rows_per_id, l.rows, l.n, l.scaling, l.scaling_value, nullptr, nullptr}; }
 int r16_of(const Lora& l) { return (l.rank + 15) / 16 * 16; }
 
 template <int MT, int NJ, int WARPS, int STAGES>
-int launch_shrink(const Lora& l, const bf16* x, int64_t stride, int cols, const bf16* f, bf16* hx, uint16_t* owners, int sms, cudaStream_t s) {
+int launch_shrink(const Lora& l, const bf16* x, int64_t stride, int cols, const bf16* f, bf16* hx, int sms, cudaStream_t s) {
   constexpr int smem = WARPS * STAGES * shrink_stage<MT, NJ>();
   static_assert(WARPS * 16 * MT * 8 * NJ * 4 <= smem, "the warps' sums");
   auto kernel = shrink_mma_kernel<MT, NJ, WARPS, STAGES>;
@@ -787,7 +761,7 @@ int launch_shrink(const Lora& l, const bf16* x, int64_t stride, int cols, const 
   const int js = (r16_of(l) + 8 * NJ - 1) / (8 * NJ);
   // where there are SMs to spare, a tile's adapters are shared out too
   const int z = (int)std::max<int64_t>(1, std::min<int64_t>({l.n, 16 * MT, l.rows, 2 * sms / std::max<int64_t>(1, tiles * js)}));
-  kernel<<<dim3((unsigned)tiles, js, z), WARPS * 32, smem, s>>>(x, stride, cols, f, l.rank, r16_of(l), rows_of(l), hx, owners);
+  kernel<<<dim3((unsigned)tiles, js, z), WARPS * 32, smem, s>>>(x, stride, cols, f, l.rank, r16_of(l), lora_rows(l), hx);
   return cuda_fail(cudaGetLastError(), "lora shrink launch");
 }
 
@@ -837,13 +811,13 @@ int tdb_lora_umma_applies(const Lora* l) {
 
 int64_t tdb_lora_inner(const Lora* l) { return 2 * r16_of(*l); }
 
-int tdb_lora_umma_shrink(const Lora* l, int back, const void* f, void* hx, uint16_t* owners, void* stream) {
+int tdb_lora_umma_shrink(const Lora* l, int back, const void* f, void* hx, void* stream) {
   int sms = 0;
   if (const int rc = device_sms(&sms)) return rc;
   const bf16* x = (const bf16*)(back ? l->dy : l->x);
   const int64_t stride = back ? l->dy_stride : l->x_stride;
   const int cols = back ? l->features : l->cols;
-  auto run = [&](auto launch) { return launch(*l, x, stride, cols, (const bf16*)f, (bf16*)hx, owners, sms, (cudaStream_t)stream); };
+  auto run = [&](auto launch) { return launch(*l, x, stride, cols, (const bf16*)f, (bf16*)hx, sms, (cudaStream_t)stream); };
   const bool few = l->rows <= 16 * sms;
   if (l->rank <= 16) return run(few ? launch_shrink<1, 2, 8, 2> : launch_shrink<2, 2, 4, 4>);
   if (l->rank <= 32) return run(few ? launch_shrink<1, 4, 8, 2> : launch_shrink<2, 4, 4, 3>);
@@ -854,7 +828,7 @@ int tdb_lora_umma_product(const Lora* l, int back, const void* f, const void* hx
   int sms = 0, rc;
   if ((rc = device_sms(&sms))) return rc;
   const int K = back ? l->features : l->cols, N = back ? l->cols : l->features;
-  const ProductParams p{rows_of(*l), (const bf16*)hx, (const bf16*)f, back ? nullptr : (const bf16*)l->bias, K, N, l->rank, r16_of(*l), (bf16*)y, status};
+  const ProductParams p{lora_rows_as_they_come(*l), (const bf16*)hx, (const bf16*)f, back ? nullptr : (const bf16*)l->bias, K, N, l->rank, r16_of(*l), (bf16*)y, status};
   const Shape shape = shape_of(l->rows, N, sms);
   CUtensorMap tx, tw, ty;
   if ((rc = bf16_map_2d(&tx, back ? l->dy : l->x, K, l->rows, back ? l->dy_stride : l->x_stride, BM, back ? "dy" : "x"))) return rc;
@@ -877,12 +851,13 @@ int tdb_lora_turn(const Lora* l, void* a_turned, void* b_turned, void* stream) {
 
 int tdb_lora_umma_gather_factors(const Lora* l) { return l->rank <= 16 ? 16 : l->rank <= 32 ? 32 : 64; }
 
-int tdb_lora_umma_gather(const Lora* l, int of_b, const void* v, const uint16_t* owners, float* part, int shares, void* stream) {
+int tdb_lora_umma_gather(const Lora* l, int of_b, const void* v, float* part, int shares, void* stream) {
   const int cols = of_b ? l->features : l->cols, r16 = r16_of(*l), mt = tdb_lora_umma_gather_factors(l) / 16, j_blocks = (r16 + 16 * mt - 1) / (16 * mt);
+  const LoraRows rows = lora_rows(*l);
   auto run = [&](auto kernel) {
     if (const int rc = opt_in_smem(reinterpret_cast<const void*>(kernel), gather_smem(mt))) return rc;
     kernel<<<dim3((cols + GC - 1) / GC, l->n * j_blocks, shares), 256, gather_smem(mt), (cudaStream_t)stream>>>(
-        (const bf16*)(of_b ? l->dy : l->x), of_b ? l->dy_stride : l->x_stride, cols, (const bf16*)v, r16, l->rank, owners, l->rows, l->n, j_blocks, part);
+        (const bf16*)(of_b ? l->dy : l->x), of_b ? l->dy_stride : l->x_stride, cols, (const bf16*)v, r16, l->rank, rows.order, rows.starts, (int)l->rows, l->n, j_blocks, part);
     return cuda_fail(cudaGetLastError(), "lora gather launch");
   };
   return mt == 1 ? run(gather_mma_kernel<1>) : mt == 2 ? run(gather_mma_kernel<2>) : run(gather_mma_kernel<4>);

@@ -191,7 +191,7 @@ int tdb_lora_skinny(const Lora* l, const void* hx, void* y, void* stream) {
   cudaStream_t s = (cudaStream_t)stream;
   int sms = 0;
   if (const int rc = device_sms(&sms)) return rc;
-  const SkinnyAdapters a{LoraRows{l->ids, l->id_bytes, l->rows_per_id, l->rows, l->n, l->scaling, l->scaling_value, nullptr, nullptr}, (const __nv_bfloat16*)hx,
+  const SkinnyAdapters a{lora_rows_as_they_come(*l), (const __nv_bfloat16*)hx,
                          (const __nv_bfloat16*)l->b, l->rank, (l->rank + 15) / 16 * 16};
   const int T = (int)l->rows;
   const cudaError_t e = T <= 16 ? launch_rows<1>(l->x, l->w, l->bias, T, l->cols, l->features, false, &a, true, y, sms, s)

@@ -155,7 +155,7 @@ struct Lora {
   const void* ids;                                    // see LoraRows
   int id_bytes;
   int64_t rows_per_id;
-  const int32_t* plan;                                // of tdb_lora_plan(), or null; for the kernels of any type and size
+  const int32_t* plan;                                // of tdb_lora_plan(), or null
 };
 }  // namespace tdb
 
@@ -198,7 +198,8 @@ TDB_HOST_API int64_t tdb_norm_partial_floats(int64_t rows, int cols);
 TDB_HOST_API int tdb_norm_backward(const tdb::Norm* n, int dtype, void* stream);
 // Adapters beside a shared product, any type and size.  back: from dy through b and a instead of from x through a and b.  h: fp32 [rows, rank].
 // base: the product alone, fp32 [rows, columns of y].  h lies in the order of l->plan, where there is one.
-TDB_HOST_API int64_t tdb_lora_plan_words(const tdb::Lora* l);
+// The rows sorted by adapter: [n + 2] first positions, [rows] rows, [rows] ids.
+TDB_HOST_API int64_t tdb_lora_plan_words(const tdb::Lora* l, int train);
 TDB_HOST_API int tdb_lora_plan(const tdb::Lora* l, int32_t* plan, void* stream);
 TDB_HOST_API int tdb_lora_shrink(const tdb::Lora* l, int back, float* h, void* stream);
 TDB_HOST_API int tdb_lora_expand(const tdb::Lora* l, int back, const float* base, const float* h, void* y, void* stream);
@@ -209,13 +210,13 @@ TDB_HOST_API int tdb_lora_gather(const tdb::Lora* l, int of_b, const float* v, f
 TDB_HOST_API int tdb_lora_gather_sum(const tdb::Lora* l, int of_b, const float* part, int shares, void* out, void* stream);
 // The same on the tensor cores (lora_umma.cu), for bf16 with columns and features that are multiples of eight, all tensors 16-byte aligned and rows no
 // less than a row apart.  f: the factors that are multiplied with x (a) or dy (b turned, [n, rank, features]) in `shrink`, and those that make y (b) or dx (a
-// turned, [n, cols, rank]) in `product`.  hx, v: bf16 [rows, tdb_lora_inner()].  status: int32[4], word 0 tells of a wait that gave up.
-// owners: [ceil(rows / 16)][n], written by `shrink` unless null, read by `gather`.
+// turned, [n, cols, rank]) in `product`.  hx, v: bf16 [rows, tdb_lora_inner()].  status: int32[4], word 0 tells of a wait that gave up.  `gather` goes by l->plan wherever the rows have ids; hx and v lie in
+// the order of the rows.
 TDB_HOST_API int tdb_lora_umma_applies(const tdb::Lora* l);
 TDB_HOST_API int64_t tdb_lora_inner(const tdb::Lora* l);
-TDB_HOST_API int tdb_lora_umma_shrink(const tdb::Lora* l, int back, const void* f, void* hx, uint16_t* owners, void* stream);
+TDB_HOST_API int tdb_lora_umma_shrink(const tdb::Lora* l, int back, const void* f, void* hx, void* stream);
 TDB_HOST_API int tdb_lora_umma_product(const tdb::Lora* l, int back, const void* f, const void* hx, void* y, int32_t* status, void* stream);
-TDB_HOST_API int tdb_lora_umma_gather(const tdb::Lora* l, int of_b, const void* v, const uint16_t* owners, float* part, int shares, void* stream);
+TDB_HOST_API int tdb_lora_umma_gather(const tdb::Lora* l, int of_b, const void* v, float* part, int shares, void* stream);
 // a and b turned, either to null where it is not needed.
 TDB_HOST_API int tdb_lora_turn(const tdb::Lora* l, void* a_turned, void* b_turned, void* stream);
 TDB_HOST_API int tdb_lora_umma_gather_factors(const tdb::Lora* l);
