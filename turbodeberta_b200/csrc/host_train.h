@@ -330,15 +330,20 @@ std::tuple<Tensor, Tensor, Tensor> run_lora(LoraCall& c, at::IntArrayRef shape, 
   return {lora_product(c, false, c.b, h, stream).view(shape), h, plan};
 }
 
-Tensor lora_gradient(const LoraCall& c, bool of_b, const Tensor& v, cudaStream_t stream) {
-  const Tensor& like = of_b ? c.b : c.a;
-  if (c.l.rows == 0) return at::zeros_like(like);
-  const int shares = tdb_lora_gather_shares(&c.l, of_b, c.tensor_cores ? tdb_lora_umma_gather_factors(&c.l) : 16);
-  Tensor part = c.floats({shares, c.l.n, c.l.rank, of_b ? c.l.features : c.l.cols}), out = at::empty(like.sizes(), like.options());
-  if (c.tensor_cores) check_rc(tdb_lora_umma_gather(&c.l, of_b, v.data_ptr(), part.data_ptr<float>(), shares, stream));
-  else check_rc(tdb_lora_gather(&c.l, of_b, v.data_ptr<float>(), part.data_ptr<float>(), shares, stream));
-  check_rc(tdb_lora_gather_sum(&c.l, of_b, part.data_ptr<float>(), shares, out.data_ptr(), stream));
-  return out;
+// (gradient of a, gradient of b), where u and h are given.
+std::pair<Tensor, Tensor> lora_gradients(const LoraCall& c, const Tensor& u, const Tensor& h, cudaStream_t stream) {
+  const int factors = c.tensor_cores ? tdb_lora_umma_gather_factors(&c.l) : 16;
+  tdb::LoraGradients g{};
+  Tensor da, db, part;
+  const int64_t of_a = (int64_t)c.l.n * c.l.rank * c.l.cols, of_b = (int64_t)c.l.n * c.l.rank * c.l.features;
+  if (u.defined()) { g.u = u.data_ptr(); g.shares_a = tdb_lora_gather_shares(&c.l, 0, factors); da = at::empty(c.a.sizes(), c.a.options()); g.da = da.data_ptr(); }
+  if (h.defined()) { g.h = h.data_ptr(); g.shares_b = tdb_lora_gather_shares(&c.l, 1, factors); db = at::empty(c.b.sizes(), c.b.options()); g.db = db.data_ptr(); }
+  part = c.floats({g.shares_a * of_a + g.shares_b * of_b});
+  if (u.defined()) g.part_a = part.data_ptr<float>();
+  if (h.defined()) g.part_b = part.data_ptr<float>() + g.shares_a * of_a;
+  check_rc(c.tensor_cores ? tdb_lora_umma_gather(&c.l, &g, stream) : tdb_lora_gather(&c.l, &g, stream));
+  check_rc(tdb_lora_gather_sum(&c.l, &g, stream));
+  return {da, db};
 }
 
 class LoraNode : public torch::autograd::Function<LoraNode> {
@@ -380,8 +385,12 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
       u = lora_shrink(c, true, b_turned, stream);
       if (need_x) dx = lora_product(c, true, a_turned, u, stream).view(x.sizes());
     }
-    if (need_a) da = lora_gradient(c, false, u, stream);
-    if (need_b) db = lora_gradient(c, true, h, stream);
+    if (c.l.rows == 0) {
+      if (need_a) da = at::zeros_like(a);
+      if (need_b) db = at::zeros_like(b);
+    } else if (need_a || need_b) {
+      std::tie(da, db) = lora_gradients(c, need_a ? u : Tensor(), need_b ? h : Tensor(), stream);
+    }
     const Tensor none;
     return {dx, none, none, da, db, none, none, none, none};
   }

@@ -43,9 +43,9 @@ __device__ __forceinline__ void find_present(Present& s, const LoraRows& rows, i
 // a fixed order too).  One block: every warp counts its share of the rows by adapter, the counts are added up adapter by adapter, and the
 // warps go through their rows once more.  plan: [bins + 1] first positions, [rows] rows, [rows] ids; bins = n + 1.
 constexpr int SORT_BYTES = 200 * 1024;
-int sort_warps(int n) { return std::min(32, SORT_BYTES / 4 / (n + 1)); }
+int sort_warps(int n) { return std::min(32, SORT_BYTES / 4 / (n + 1) - 1); }
 __global__ void __launch_bounds__(1024) sort_kernel(LoraRows rows, int32_t* __restrict__ plan) {
-  extern __shared__ int counts[];                    // [warps][bins]
+  extern __shared__ int counts[];                    // [warps][bins], then the bins' own sums
   __shared__ int sums[32];
   const int warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32, bins = rows.n + 1;
   int* mine = counts + warp * bins;
@@ -54,23 +54,43 @@ __global__ void __launch_bounds__(1024) sort_kernel(LoraRows rows, int32_t* __re
   for (int i = lane; i < bins; i += 32) mine[i] = 0;
   __syncwarp();
   auto walk = [&](auto&& step) {
-    for (int64_t t0 = begin; t0 < end; t0 += 32) {
-      const bool in = t0 + lane < end;
-      const int id = in ? adapter_of(rows, t0 + lane) : -1, bin = in ? (id < 0 ? rows.n : id) : -1;
-      const uint32_t same = __match_any_sync(0xffffffffu, bin), before = same & ((1u << lane) - 1u);
-      if (in) step(t0 + lane, id, bin, __popc(before));
-      __syncwarp();
-      if (in && before == 0) mine[bin] += __popc(same);
-      __syncwarp();
+    constexpr int AT_ONCE = 8;                       // loads on their way together
+    for (int64_t t0 = begin; t0 < end; t0 += 32 * AT_ONCE) {
+      int id[AT_ONCE];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) id[i] = t0 + 32 * i + lane < end ? adapter_of(rows, t0 + 32 * i + lane) : -1;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int64_t row = t0 + 32 * i + lane;
+        const bool in = row < end;
+        const int bin = in ? (id[i] < 0 ? rows.n : id[i]) : -1;
+        const uint32_t same = __match_any_sync(0xffffffffu, bin), before = same & ((1u << lane) - 1u);
+        if (in) step(row, id[i], bin, __popc(before));
+        __syncwarp();
+        if (in && before == 0) mine[bin] += __popc(same);
+        __syncwarp();
+      }
     }
   };
   walk([](int64_t, int, int, int) {});
   __syncthreads();
-  // exclusive sums, adapter by adapter and within one warp by warp; a thread has neighbouring bins
+  // exclusive sums, warp by warp within a bin, then bin by bin
+  int* bases = counts + warps * bins;
+  for (int i = warp; i < bins; i += warps) {
+    const int n = lane < warps ? counts[lane * bins + i] : 0;
+    int run = n;
+#pragma unroll
+    for (int off = 1; off < 32; off *= 2) {
+      const int o = __shfl_up_sync(0xffffffffu, run, off);
+      if (lane >= off) run += o;
+    }
+    if (lane < warps) counts[lane * bins + i] = run - n;
+    if (lane == 31) bases[i] = run;
+  }
+  __syncthreads();
   const int each = (bins + blockDim.x - 1) / blockDim.x, first = threadIdx.x * each, last = min(bins, first + each);
   int total = 0;
-  for (int i = first; i < last; ++i)
-    for (int w = 0; w < warps; ++w) total += counts[w * bins + i];
+  for (int i = first; i < last; ++i) total += bases[i];
   int run = total;
 #pragma unroll
   for (int off = 1; off < 32; off *= 2) {
@@ -82,17 +102,14 @@ __global__ void __launch_bounds__(1024) sort_kernel(LoraRows rows, int32_t* __re
   int base = run - total;
   for (int w = 0; w < warp; ++w) base += sums[w];
   for (int i = first; i < last; ++i) {
-    plan[i] = base;
-    for (int w = 0; w < warps; ++w) {
-      const int n = counts[w * bins + i];
-      counts[w * bins + i] = base;
-      base += n;
-    }
+    const int n = bases[i];
+    plan[i] = bases[i] = base;
+    base += n;
   }
   if (threadIdx.x == 0) plan[bins] = (int)rows.rows;
   __syncthreads();
   walk([&](int64_t row, int id, int bin, int rank) {
-    const int at = mine[bin] + rank;
+    const int at = bases[bin] + mine[bin] + rank;
     order[at] = (int32_t)row;
     ids[at] = id;
   });
@@ -229,17 +246,25 @@ __global__ void __launch_bounds__(COLS) expand_kernel(const float* base, const T
     if (t0 + r < rows.rows) put(y + place[r] + c, sum[r] + b + acc[r]);
 }
 
-// part[z][a][j][c] = sum over this share of the rows t of adapter a of v[t][j] x[t][c].  A block: one adapter, 16 factors, 128 columns.
+// part[z][a][j][c] = sum over a share of the rows t of adapter a of v[t][j] x[t][c].  A block: one adapter, 16 factors, 128 columns, of one of the
+// two gradients (blockIdx.x: the blocks of columns of the first, then those of the second).
+template <typename T> struct Side { const T* x; int64_t stride; int cols; const float* v; float* part; int blocks, shares; };
 template <typename T>
-__global__ void __launch_bounds__(COLS) gather_kernel(const T* __restrict__ x, int64_t stride, int cols, const float* __restrict__ v, int rank,
-                                                      LoraRows rows, int j_blocks, float* __restrict__ part) {
+__global__ void __launch_bounds__(COLS) gather_kernel(Side<T> one, Side<T> two, int rank, LoraRows rows, int j_blocks) {
+  const bool later = (int)blockIdx.x >= one.blocks;
+  const Side<T> side = later ? two : one;
+  const T* __restrict__ x = side.x;
+  const float* __restrict__ v = side.v;
+  const int64_t stride = side.stride;
+  const int cols = side.cols;
+  if ((int)blockIdx.z >= side.shares) return;
   __shared__ int ids[32];
   __shared__ int64_t place[32];
   __shared__ __align__(16) float vs[32][16];
-  const int a = blockIdx.y / j_blocks, j0 = blockIdx.y % j_blocks * 16, jn = min(16, rank - j0), c = blockIdx.x * COLS + threadIdx.x;
+  const int a = blockIdx.y / j_blocks, j0 = blockIdx.y % j_blocks * 16, jn = min(16, rank - j0), c = (blockIdx.x - (later ? one.blocks : 0)) * COLS + threadIdx.x;
   // sorted rows: a share of the adapter's own positions, otherwise of all
   const int64_t first = rows.starts ? rows.starts[a] : 0, last = rows.starts ? rows.starts[a + 1] : rows.rows;
-  const int64_t share = ((last - first + gridDim.z - 1) / gridDim.z + 31) / 32 * 32, begin = first + blockIdx.z * share, end = min(last, begin + share);
+  const int64_t share = ((last - first + side.shares - 1) / side.shares + 31) / 32 * 32, begin = first + blockIdx.z * share, end = min(last, begin + share);
   float acc[16];
 #pragma unroll
   for (int j = 0; j < 16; ++j) acc[j] = 0.f;
@@ -273,32 +298,37 @@ __global__ void __launch_bounds__(COLS) gather_kernel(const T* __restrict__ x, i
   const int n = gridDim.y / j_blocks;
 #pragma unroll
   for (int j = 0; j < 16; ++j)
-    if (j < jn) part[(((int64_t)blockIdx.z * n + a) * rank + j0 + j) * cols + c] = acc[j];
+    if (j < jn) side.part[(((int64_t)blockIdx.z * n + a) * rank + j0 + j) * cols + c] = acc[j];
 }
 
-// The shares' sum, as [a][j][c] or, turned by pieces of 8 x 32, [a][c][j].
+// The shares' sums: of a's gradient as [a][j][c], of b's turned by pieces of 8 x 32 to [a][c][j].
+template <typename T> struct Sum { const float* part; T* out; int shares, blocks, cols; };
 template <typename T>
-__global__ void __launch_bounds__(256) gather_sum_kernel(const float* __restrict__ part, int shares, int64_t total, T* __restrict__ out) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= total) return;
-  float s = 0.f;
-#pragma unroll 8
-  for (int z = 0; z < shares; ++z) s += part[z * total + e];
-  put(out + e, s);
-}
-template <typename T>
-__global__ void __launch_bounds__(256) gather_sum_turned_kernel(const float* __restrict__ part, int shares, int64_t total, int rank, int cols, T* __restrict__ out) {
+__global__ void __launch_bounds__(256) gather_sum_kernel(Sum<T> of_a, Sum<T> of_b, int n, int rank) {
   __shared__ float s[8][33];
-  const int64_t a = blockIdx.z;
-  const int c0 = blockIdx.x * 32, j0 = blockIdx.y * 8, tx = threadIdx.x % 32, ty = threadIdx.x / 32;
-  float v = 0.f;
-  if (j0 + ty < rank && c0 + tx < cols)
+  const bool turned = (int)blockIdx.x >= of_a.blocks;
+  const Sum<T> sum = turned ? of_b : of_a;
+  const int64_t total = (int64_t)n * rank * sum.cols;
+  if (!turned) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= total) return;
+    float v = 0.f;
 #pragma unroll 8
-    for (int z = 0; z < shares; ++z) v += part[z * total + (a * rank + j0 + ty) * cols + c0 + tx];
+    for (int z = 0; z < sum.shares; ++z) v += sum.part[z * total + e];
+    put(sum.out + e, v);
+    return;
+  }
+  const int across = (sum.cols + 31) / 32, down = (rank + 7) / 8, block = blockIdx.x - of_a.blocks;
+  const int64_t a = block / (across * down);
+  const int c0 = block % across * 32, j0 = block / across % down * 8, tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  float v = 0.f;
+  if (j0 + ty < rank && c0 + tx < sum.cols)
+#pragma unroll 8
+    for (int z = 0; z < sum.shares; ++z) v += sum.part[z * total + (a * rank + j0 + ty) * sum.cols + c0 + tx];
   s[ty][tx] = v;
   __syncthreads();
   const int c = threadIdx.x / 8, j = threadIdx.x % 8;
-  if (j0 + j < rank && c0 + c < cols) put(out + (a * cols + c0 + c) * rank + j0 + j, s[j][c]);
+  if (j0 + j < rank && c0 + c < sum.cols) put(sum.out + (a * sum.cols + c0 + c) * rank + j0 + j, s[j][c]);
 }
 
 template <typename T>
@@ -321,18 +351,20 @@ int expand(const Lora& l, bool back, const float* base, const float* h, void* y,
   return cuda_fail(cudaGetLastError(), "lora expand launch");
 }
 template <typename T>
-int gather(const Lora& l, bool of_b, const float* v, float* part, int shares, cudaStream_t s) {
-  const int cols = of_b ? l.features : l.cols, j_blocks = (l.rank + 15) / 16;
-  const dim3 grid((cols + COLS - 1) / COLS, l.n * j_blocks, shares);
-  gather_kernel<T><<<grid, COLS, 0, s>>>((const T*)(of_b ? l.dy : l.x), of_b ? l.dy_stride : l.x_stride, cols, v, l.rank, lora_rows(l), j_blocks, part);
+int gather(const Lora& l, const LoraGradients& g, cudaStream_t s) {
+  auto side = [&](const void* x, int64_t stride, int cols, const void* v, float* part, int shares) {
+    return Side<T>{(const T*)x, stride, cols, (const float*)v, part, part ? (cols + COLS - 1) / COLS : 0, shares};
+  };
+  const int j_blocks = (l.rank + 15) / 16;
+  const Side<T> a = side(l.x, l.x_stride, l.cols, g.u, g.part_a, g.shares_a), b = side(l.dy, l.dy_stride, l.features, g.h, g.part_b, g.shares_b);
+  gather_kernel<T><<<dim3(a.blocks + b.blocks, l.n * j_blocks, std::max(a.shares, b.shares)), COLS, 0, s>>>(a, b, l.rank, lora_rows(l), j_blocks);
   return cuda_fail(cudaGetLastError(), "lora gather launch");
 }
 template <typename T>
-int gather_sum(const Lora& l, bool of_b, const float* part, int shares, void* out, cudaStream_t s) {
-  const int cols = of_b ? l.features : l.cols;
-  const int64_t total = (int64_t)l.n * l.rank * cols;
-  if (of_b) gather_sum_turned_kernel<T><<<dim3((cols + 31) / 32, (l.rank + 7) / 8, l.n), 256, 0, s>>>(part, shares, total, l.rank, cols, (T*)out);
-  else gather_sum_kernel<T><<<(unsigned)((total + 255) / 256), 256, 0, s>>>(part, shares, total, (T*)out);
+int gather_sum(const Lora& l, const LoraGradients& g, cudaStream_t s) {
+  const int64_t each = (int64_t)l.n * l.rank * l.cols, pieces = (int64_t)l.n * ((l.features + 31) / 32) * ((l.rank + 7) / 8);
+  const Sum<T> a{g.part_a, (T*)g.da, g.shares_a, g.part_a ? (int)((each + 255) / 256) : 0, l.cols}, b{g.part_b, (T*)g.db, g.shares_b, g.part_b ? (int)pieces : 0, l.features};
+  gather_sum_kernel<T><<<a.blocks + b.blocks, 256, 0, s>>>(a, b, l.n, l.rank);
   return cuda_fail(cudaGetLastError(), "lora gather sum launch");
 }
 
@@ -351,7 +383,7 @@ int64_t tdb_lora_plan_words(const Lora* l, int train) {
   return wanted && l->rows < (int64_t)1 << 30 ? l->n + 2 + 2 * l->rows : 0;
 }
 int tdb_lora_plan(const Lora* l, int32_t* plan, void* stream) {
-  const int warps = sort_warps(l->n), smem = warps * (l->n + 1) * 4;
+  const int warps = sort_warps(l->n), smem = (warps + 1) * (l->n + 1) * 4;
   if (smem > 48 * 1024)
     if (const int rc = opt_in_smem(reinterpret_cast<const void*>(sort_kernel), SORT_BYTES)) return rc;
   Lora plain = *l;
@@ -374,12 +406,11 @@ int tdb_lora_shrink(const Lora* l, int back, float* h, void* stream) {
 int tdb_lora_expand(const Lora* l, int back, const float* base, const float* h, void* y, void* stream) {
   return l->dtype == TDB_DTYPE_F32 ? expand<float>(*l, back, base, h, y, (cudaStream_t)stream) : expand<__nv_bfloat16>(*l, back, base, h, y, (cudaStream_t)stream);
 }
-int tdb_lora_gather(const Lora* l, int of_b, const float* v, float* part, int shares, void* stream) {
-  return l->dtype == TDB_DTYPE_F32 ? gather<float>(*l, of_b, v, part, shares, (cudaStream_t)stream) : gather<__nv_bfloat16>(*l, of_b, v, part, shares, (cudaStream_t)stream);
+int tdb_lora_gather(const Lora* l, const LoraGradients* g, void* stream) {
+  return l->dtype == TDB_DTYPE_F32 ? gather<float>(*l, *g, (cudaStream_t)stream) : gather<__nv_bfloat16>(*l, *g, (cudaStream_t)stream);
 }
-int tdb_lora_gather_sum(const Lora* l, int of_b, const float* part, int shares, void* out, void* stream) {
-  return l->dtype == TDB_DTYPE_F32 ? gather_sum<float>(*l, of_b, part, shares, out, (cudaStream_t)stream)
-                                   : gather_sum<__nv_bfloat16>(*l, of_b, part, shares, out, (cudaStream_t)stream);
+int tdb_lora_gather_sum(const Lora* l, const LoraGradients* g, void* stream) {
+  return l->dtype == TDB_DTYPE_F32 ? gather_sum<float>(*l, *g, (cudaStream_t)stream) : gather_sum<__nv_bfloat16>(*l, *g, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -636,23 +636,31 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
 // ------------------------------------------------------------------------------------------------------------------- gather
 // part[z][a][j][c] = sum over a share of the rows t of adapter a of v[t][j] x[t][c], v being the sum of two bf16 numbers.  A block: one
 // adapter, 16 MT factors, 128 columns; a warp: 16 columns.  The adapter's rows, which the plan lists, come in tiles of 64 through shared memory, two at
-// a time; blockIdx.z takes every gridDim.z-th tile.  Bound by reading x.
+// a time; blockIdx.z takes every shares-th tile.  Both gradients in one launch (blockIdx.x: the blocks of columns of the first, then those of the
+// second).  Bound by reading x.
 constexpr int GC = 128, GP = GC + 8, G_BATCH = 16;     // G_BATCH: tiles whose rows are looked up at once
 __host__ __device__ constexpr int gather_pitch(int mt) { return 32 * mt + 8; }
 __host__ __device__ constexpr int gather_smem(int mt) { return 2 * 64 * (GP + gather_pitch(mt)) * 2; }
 
+struct GatherSide { const bf16* x; int64_t stride; int cols; const bf16* v; float* part; int blocks, shares; };
+
 template <int MT>
-__global__ void __launch_bounds__(256) gather_mma_kernel(const bf16* __restrict__ x, int64_t stride, int cols, const bf16* __restrict__ v, int r16, int rank,
-                                                         const int32_t* __restrict__ order, const int32_t* __restrict__ starts, int rows, int n_adapters, int j_blocks,
-                                                         float* __restrict__ part) {
+__global__ void __launch_bounds__(256) gather_mma_kernel(const GatherSide one, const GatherSide two, int r16, int rank, const int32_t* __restrict__ order,
+                                                         const int32_t* __restrict__ starts, int rows, int n_adapters, int j_blocks) {
   constexpr int VP = gather_pitch(MT);
+  const bool later = (int)blockIdx.x >= one.blocks;
+  const GatherSide side = later ? two : one;
+  const bf16 *__restrict__ x = side.x, *__restrict__ v = side.v;
+  const int64_t stride = side.stride;
+  const int cols = side.cols, shares = side.shares;
+  if ((int)blockIdx.z >= shares) return;
   extern __shared__ __align__(16) bf16 tiles[];
   __shared__ int place[G_BATCH * 64];                  // -1: behind the adapter's last row
   bf16 *xs[2] = {tiles, tiles + 64 * GP}, *vs[2] = {tiles + 2 * 64 * GP, tiles + 2 * 64 * GP + 64 * VP};
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int a = blockIdx.y / j_blocks, j0 = blockIdx.y % j_blocks * 16 * MT, c0 = blockIdx.x * GC;
+  const int a = blockIdx.y / j_blocks, j0 = blockIdx.y % j_blocks * 16 * MT, c0 = (blockIdx.x - (later ? one.blocks : 0)) * GC;
   const int first = starts ? starts[a] : 0, last = starts ? starts[a + 1] : rows, all = (last - first + 63) / 64;
-  const int mine = all > (int)blockIdx.z ? (all - blockIdx.z + gridDim.z - 1) / gridDim.z : 0;       // tiles of this block
+  const int mine = all > (int)blockIdx.z ? (all - (int)blockIdx.z + shares - 1) / shares : 0;       // tiles of this block
   float acc[MT][2][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -668,7 +676,7 @@ __global__ void __launch_bounds__(256) gather_mma_kernel(const bf16* __restrict_
     const int todo = min(G_BATCH, mine - batch);
     __syncthreads();
     for (int e = tid; e < todo * 64; e += 256) {
-      const int at = first + ((batch + e / 64) * gridDim.z + blockIdx.z) * 64 + e % 64;
+      const int at = first + ((batch + e / 64) * shares + (int)blockIdx.z) * 64 + e % 64;
       place[e] = at >= last ? -1 : order ? order[at] : at;
     }
     __syncthreads();
@@ -724,7 +732,7 @@ __global__ void __launch_bounds__(256) gather_mma_kernel(const bf16* __restrict_
       for (int e = 0; e < 2; ++e) {
         const int c = c0 + warp * 16 + 8 * e + 2 * t;
         if (c < cols)
-          *reinterpret_cast<float2*>(part + (((int64_t)blockIdx.z * n_adapters + a) * rank + j) * cols + c) = make_float2(acc[m][e][2 * r], acc[m][e][2 * r + 1]);
+          *reinterpret_cast<float2*>(side.part + (((int64_t)blockIdx.z * n_adapters + a) * rank + j) * cols + c) = make_float2(acc[m][e][2 * r], acc[m][e][2 * r + 1]);
       }
     }
 }
@@ -851,13 +859,17 @@ int tdb_lora_turn(const Lora* l, void* a_turned, void* b_turned, void* stream) {
 
 int tdb_lora_umma_gather_factors(const Lora* l) { return l->rank <= 16 ? 16 : l->rank <= 32 ? 32 : 64; }
 
-int tdb_lora_umma_gather(const Lora* l, int of_b, const void* v, float* part, int shares, void* stream) {
-  const int cols = of_b ? l->features : l->cols, r16 = r16_of(*l), mt = tdb_lora_umma_gather_factors(l) / 16, j_blocks = (r16 + 16 * mt - 1) / (16 * mt);
+int tdb_lora_umma_gather(const Lora* l, const LoraGradients* g, void* stream) {
+  auto side = [](const void* x, int64_t stride, int cols, const void* v, float* part, int shares) {
+    return GatherSide{(const bf16*)x, stride, cols, (const bf16*)v, part, part ? (cols + GC - 1) / GC : 0, shares};
+  };
+  const GatherSide a = side(l->x, l->x_stride, l->cols, g->u, g->part_a, g->shares_a), b = side(l->dy, l->dy_stride, l->features, g->h, g->part_b, g->shares_b);
+  const int r16 = r16_of(*l), mt = tdb_lora_umma_gather_factors(l) / 16, j_blocks = (r16 + 16 * mt - 1) / (16 * mt);
   const LoraRows rows = lora_rows(*l);
   auto run = [&](auto kernel) {
     if (const int rc = opt_in_smem(reinterpret_cast<const void*>(kernel), gather_smem(mt))) return rc;
-    kernel<<<dim3((cols + GC - 1) / GC, l->n * j_blocks, shares), 256, gather_smem(mt), (cudaStream_t)stream>>>(
-        (const bf16*)(of_b ? l->dy : l->x), of_b ? l->dy_stride : l->x_stride, cols, (const bf16*)v, r16, l->rank, rows.order, rows.starts, (int)l->rows, l->n, j_blocks, part);
+    kernel<<<dim3(a.blocks + b.blocks, l->n * j_blocks, std::max(a.shares, b.shares)), 256, gather_smem(mt), (cudaStream_t)stream>>>(
+        a, b, r16, l->rank, rows.order, rows.starts, (int)l->rows, l->n, j_blocks);
     return cuda_fail(cudaGetLastError(), "lora gather launch");
   };
   return mt == 1 ? run(gather_mma_kernel<1>) : mt == 2 ? run(gather_mma_kernel<2>) : run(gather_mma_kernel<4>);

@@ -157,6 +157,13 @@ struct Lora {
   int64_t rows_per_id;
   const int32_t* plan;                                // of tdb_lora_plan(), or null
 };
+// The gradients of a, from u and x, and of b, from h and dy; either with part null where it is not wanted.
+struct LoraGradients {
+  const void *u, *h;
+  float *part_a, *part_b;                             // [shares][n][rank][columns]
+  int shares_a, shares_b;                             // tdb_lora_gather_shares(), 0 without part
+  void *da, *db;
+};
 }  // namespace tdb
 
 // What the host extension calls (the checks and the launch behind the tdb_attn_fwd_* entry points on a filled AttnParams,
@@ -203,20 +210,19 @@ TDB_HOST_API int64_t tdb_lora_plan_words(const tdb::Lora* l, int train);
 TDB_HOST_API int tdb_lora_plan(const tdb::Lora* l, int32_t* plan, void* stream);
 TDB_HOST_API int tdb_lora_shrink(const tdb::Lora* l, int back, float* h, void* stream);
 TDB_HOST_API int tdb_lora_expand(const tdb::Lora* l, int back, const float* base, const float* h, void* y, void* stream);
-// The gradient of a (from v = u and x) or of b (from v = h and dy).  part: [shares, n, rank, columns] floats.  factors: of a block, 16 here.
+// Sums over the rows, in shares, and the shares' sums in the type and layout of a and b.  factors: of a block, 16 here.
 TDB_HOST_API int tdb_lora_gather_shares(const tdb::Lora* l, int of_b, int factors);
-TDB_HOST_API int tdb_lora_gather(const tdb::Lora* l, int of_b, const float* v, float* part, int shares, void* stream);
-// The sum of gather's shares, to the type and layout of a (or of b).
-TDB_HOST_API int tdb_lora_gather_sum(const tdb::Lora* l, int of_b, const float* part, int shares, void* out, void* stream);
+TDB_HOST_API int tdb_lora_gather(const tdb::Lora* l, const tdb::LoraGradients* g, void* stream);
+TDB_HOST_API int tdb_lora_gather_sum(const tdb::Lora* l, const tdb::LoraGradients* g, void* stream);
 // The same on the tensor cores (lora_umma.cu), for bf16 with columns and features that are multiples of eight, all tensors 16-byte aligned and rows no
 // less than a row apart.  f: the factors that are multiplied with x (a) or dy (b turned, [n, rank, features]) in `shrink`, and those that make y (b) or dx (a
-// turned, [n, cols, rank]) in `product`.  hx, v: bf16 [rows, tdb_lora_inner()].  status: int32[4], word 0 tells of a wait that gave up.  `gather` goes by l->plan wherever the rows have ids; hx and v lie in
+// turned, [n, cols, rank]) in `product`.  hx, u, h: bf16 [rows, tdb_lora_inner()].  status: int32[4], word 0 tells of a wait that gave up.  `gather` goes by l->plan wherever the rows have ids; they lie in
 // the order of the rows.
 TDB_HOST_API int tdb_lora_umma_applies(const tdb::Lora* l);
 TDB_HOST_API int64_t tdb_lora_inner(const tdb::Lora* l);
 TDB_HOST_API int tdb_lora_umma_shrink(const tdb::Lora* l, int back, const void* f, void* hx, void* stream);
 TDB_HOST_API int tdb_lora_umma_product(const tdb::Lora* l, int back, const void* f, const void* hx, void* y, int32_t* status, void* stream);
-TDB_HOST_API int tdb_lora_umma_gather(const tdb::Lora* l, int of_b, const void* v, float* part, int shares, void* stream);
+TDB_HOST_API int tdb_lora_umma_gather(const tdb::Lora* l, const tdb::LoraGradients* g, void* stream);
 // a and b turned, either to null where it is not needed.
 TDB_HOST_API int tdb_lora_turn(const tdb::Lora* l, void* a_turned, void* b_turned, void* stream);
 TDB_HOST_API int tdb_lora_umma_gather_factors(const tdb::Lora* l);
