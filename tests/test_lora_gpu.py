@@ -230,3 +230,60 @@ def test_many_tiles_and_many_adapters_to_a_tile(rows, cols, features, rank, n, s
         assert torch.isfinite(got[k]).all()
     from turbodeberta_b200.ops.flash_attention import check_pending_status
     check_pending_status()
+
+
+FRESH = """
+import torch
+from turbodeberta_b200.ops.flash_attention import check_pending_status
+from turbodeberta_b200.ops.lora import lora_linear
+g = torch.Generator("cuda").manual_seed(0)
+r = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16()
+x, w, a, b = r(300, 128), r(192, 128), r(2, 8, 128), r(2, 192, 8)
+ids = torch.randint(-1, 2, (300,), device="cuda", generator=g)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = lora_linear(x, w, None, a, b, 0.5, ids)
+graph.replay()
+want = lora_linear(x, w, None, a, b, 0.5, ids)
+torch.cuda.synchronize()
+assert torch.equal(y, want) and torch.isfinite(y).all()
+check_pending_status()
+print("fine")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FRESH], cwd=root, capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+def test_calls_from_several_threads_and_streams():
+    """Each thread with a stream of its own, at once: the results of calls one after the other."""
+    import threading
+    problems = [problem(400, 256, 320, 16, 5, B, "texts", seed=i) for i in range(4)]
+    want = [run(p) for p in problems]
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i] = run(problems[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for w, g in zip(want, got):
+        assert all(torch.equal(w[k], g[k]) for k in w)

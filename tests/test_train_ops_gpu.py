@@ -295,3 +295,14 @@ def test_inputs_on_two_streams_and_a_captured_step():
         y2, dx2 = step(other)
     torch.cuda.synchronize()
     assert torch.equal(y, y2) and torch.equal(dx, dx2)
+
+
+@pytest.mark.parametrize("p", [0.0, 0.3])
+def test_one_tensor_as_both_summands(p):
+    """x and residual the same tensor: its gradient is the sum of both."""
+    x, _, w, b, dy = norm_case(40, 264, F, F, False)
+    both = x.clone().requires_grad_()
+    got, = torch.autograd.grad(dropout_add_layer_norm(both, both, w, b, 1e-6, p, 3), both, dy)
+    one, two = x.clone().requires_grad_(), x.clone().requires_grad_()
+    parts = torch.autograd.grad(dropout_add_layer_norm(one, two, w, b, 1e-6, p, 3), (one, two), dy)
+    assert torch.equal(got, parts[0] + parts[1])
