@@ -183,9 +183,9 @@ __global__ void __launch_bounds__(WARPS * 32) shrink_mma_kernel(const bf16* __re
 
 // ------------------------------------------------------------------------------------------------------------------ product
 // Persistent, tiles of 128 CTAS rows and BN columns, two accumulators.  With CTAS = 2 a pair of SMs works on one tile: each fetches its own
-// 128 rows of x and half of the columns of W, and the tensor cores of both read the other half from the neighbour.  That halves what has to come
-// from L2 for W, which is what bounds the product: with a 128 x 256 tile to one SM every 128 x 256 x 64 step fetched 48 KB, 12 TB/s over the
-// chip, and ran at 46 % of the tensor cores' rate (9216 rows 1024 -> 4096 without adapters: 89.9 us).
+// 128 rows of x and half of the columns of W, and the tensor cores of both read the other half from the neighbour.  That halves what W takes of L2
+// and of shared memory: 9216 rows 1024 -> 4096 without adapters take 74 us with a 128 x 256 tile to one SM and 52 with 256 x 256 to a pair, on
+// rings of 192 KB (59 with the two stages that the adapters have of it; the library's product takes 57).
 //
 // Warp 0 fetches tiles of x and W by TMA into a ring of stages, warps 2..5 fill two stages of their own with the adapters' tiles, warp 1 (of
 // the pair's first CTA) issues the products, warps 6..9 drain one accumulator (tensor memory, bias, bf16, shared memory, TMA) while the other one
@@ -790,12 +790,13 @@ int launch_product(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorM
   return cuda_fail(cudaLaunchKernelEx(&cfg, kernel, tx, tw, ty, p), "lora product launch");
 }
 
-// Columns of a tile, and whether a pair of SMs shares it: the form whose waves of tiles take least, in the time of a step.  A pair's
-// 256 x 256 tile counts 256; 128 x 128 to one SM, which waits for L2, 224; 128 x 64 176.
+// Columns of a tile, and whether a pair of SMs shares it: the form whose waves of tiles take least.  us of a launch by waves, inner dimension 4096:
+// 256 x 256 to a pair 25..27, 49..56, 83 (one, two, three); 128 x 128 to one SM 19..25, 43, 64..78 (three, four); 128 x 64 19, 37..39, 72 (four).
+// Per wave that is 256 to 195 to 175.  1024 rows 4096 -> 4096: pair 33, 43 and 69 with one SM to a tile; 512 rows 27, 25, 37; 200 rows 25, 21, 20.
 struct Shape { int columns, ctas; };
 Shape shape_of(int64_t rows, int N, int sms) {
   auto waves = [&](int m, int n, int workers) { return ((rows + m - 1) / m * ((N + n - 1) / n) + workers - 1) / workers; };
-  const int64_t pair = waves(256, 256, sms / 2) * 256, wide = waves(128, 128, sms) * 224, narrow = waves(128, 64, sms) * 176;
+  const int64_t pair = waves(256, 256, sms / 2) * 256, wide = waves(128, 128, sms) * 195, narrow = waves(128, 64, sms) * 175;
   return pair <= wide && pair <= narrow ? Shape{256, 2} : wide <= narrow ? Shape{128, 1} : Shape{64, 1};
 }
 
