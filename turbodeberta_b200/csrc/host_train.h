@@ -375,13 +375,15 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
     if (c.l.rows == 0) {
       if (need_x) dx = at::empty(x.sizes(), x.options());
     } else if (need_x || need_a) {
-      // the product may start beside the kernel in front of it, which therefore is the one that makes u
       Tensor a_turned, b_turned;
       if (c.tensor_cores) {
-        if (need_x) a_turned = at::empty({c.l.n, c.l.cols, c.l.rank}, a.options());
-        b_turned = at::empty({c.l.n, c.l.rank, c.l.features}, b.options());
+        const int64_t of_a = need_x ? a.numel() : 0;
+        const Tensor both = at::empty({of_a + b.numel()}, a.options());
+        if (need_x) a_turned = both.narrow(0, 0, of_a);
+        b_turned = both.narrow(0, of_a, b.numel());
         check_rc(tdb_lora_turn(&c.l, need_x ? a_turned.data_ptr() : nullptr, b_turned.data_ptr(), stream));
       }
+      // the product may start beside the kernel in front of it, which therefore is the one that makes u
       u = lora_shrink(c, true, b_turned, stream);
       if (need_x) dx = lora_product(c, true, a_turned, u, stream).view(x.sizes());
     }

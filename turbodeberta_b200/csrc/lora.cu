@@ -375,12 +375,11 @@ using namespace tdb;
 
 extern "C" {
 
-// Words of the plan that puts the rows in their adapters' order, 0 where there is none.  The tensor cores' gradients want it (`train`) wherever rows have
-// ids; the other kernels from 256 rows and two adapters on (a training step of 700 rows in long requests of three adapters, fp32: 124 us without,
-// 128 with).
+// Words of the plan that puts the rows in their adapters' order, 0 where there is none: with one adapter for all, and for few rows, where the launch
+// costs more than it saves (a training step of 700 rows in long requests of three adapters, fp32: 124 us without, 128 with).  Products on the
+// tensor cores go by the rows as they come; their gradients (`train`) want the plan from more rows on.
 int64_t tdb_lora_plan_words(const Lora* l, int train) {
-  const bool wanted = train ? l->ids != nullptr : l->n > 1 && l->rows >= 256;
-  return wanted && l->rows < (int64_t)1 << 30 ? l->n + 2 + 2 * l->rows : 0;
+  return l->ids && l->n > 1 && l->rows >= (train ? 768 : 256) && l->rows < (int64_t)1 << 30 ? l->n + 2 + 2 * l->rows : 0;
 }
 int tdb_lora_plan(const Lora* l, int32_t* plan, void* stream) {
   const int warps = sort_warps(l->n), smem = (warps + 1) * (l->n + 1) * 4;

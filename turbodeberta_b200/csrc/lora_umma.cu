@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
 // ------------------------------------------------------------------------------------------------------------------- gather
 // part[z][a][j][c] = sum over a share of the rows t of adapter a of v[t][j] x[t][c], v being the sum of two bf16 numbers.  A block: one
 // adapter, 16 MT factors, 128 columns; a warp: 16 columns.  The adapter's rows, which the plan lists, come in tiles of 64 through shared memory, two at
-// a time; blockIdx.z takes every shares-th tile.  Both gradients in one launch (blockIdx.x: the blocks of columns of the first, then those of the
+// a time; blockIdx.z takes every shares-th tile.  Without a plan (few rows) all rows do, zeros in the place of those that are not the adapter's.  Both gradients in one launch (blockIdx.x: the blocks of columns of the first, then those of the
 // second).  Bound by reading x.
 constexpr int GC = 128, GP = GC + 8, G_BATCH = 16;     // G_BATCH: tiles whose rows are looked up at once
 __host__ __device__ constexpr int gather_pitch(int mt) { return 32 * mt + 8; }
@@ -645,8 +645,7 @@ __host__ __device__ constexpr int gather_smem(int mt) { return 2 * 64 * (GP + ga
 struct GatherSide { const bf16* x; int64_t stride; int cols; const bf16* v; float* part; int blocks, shares; };
 
 template <int MT>
-__global__ void __launch_bounds__(256) gather_mma_kernel(const GatherSide one, const GatherSide two, int r16, int rank, const int32_t* __restrict__ order,
-                                                         const int32_t* __restrict__ starts, int rows, int n_adapters, int j_blocks) {
+__global__ void __launch_bounds__(256) gather_mma_kernel(const GatherSide one, const GatherSide two, int r16, int rank, const LoraRows rows, int j_blocks) {
   constexpr int VP = gather_pitch(MT);
   const bool later = (int)blockIdx.x >= one.blocks;
   const GatherSide side = later ? two : one;
@@ -655,11 +654,11 @@ __global__ void __launch_bounds__(256) gather_mma_kernel(const GatherSide one, c
   const int cols = side.cols, shares = side.shares;
   if ((int)blockIdx.z >= shares) return;
   extern __shared__ __align__(16) bf16 tiles[];
-  __shared__ int place[G_BATCH * 64];                  // -1: behind the adapter's last row
+  __shared__ int place[G_BATCH * 64];                  // -1: not a row of the adapter
   bf16 *xs[2] = {tiles, tiles + 64 * GP}, *vs[2] = {tiles + 2 * 64 * GP, tiles + 2 * 64 * GP + 64 * VP};
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int a = blockIdx.y / j_blocks, j0 = blockIdx.y % j_blocks * 16 * MT, c0 = (blockIdx.x - (later ? one.blocks : 0)) * GC;
-  const int first = starts ? starts[a] : 0, last = starts ? starts[a + 1] : rows, all = (last - first + 63) / 64;
+  const int first = rows.starts ? rows.starts[a] : 0, last = rows.starts ? rows.starts[a + 1] : (int)rows.rows, all = (last - first + 63) / 64;
   const int mine = all > (int)blockIdx.z ? (all - (int)blockIdx.z + shares - 1) / shares : 0;       // tiles of this block
   float acc[MT][2][4];
 #pragma unroll
@@ -677,7 +676,7 @@ __global__ void __launch_bounds__(256) gather_mma_kernel(const GatherSide one, c
     __syncthreads();
     for (int e = tid; e < todo * 64; e += 256) {
       const int at = first + ((batch + e / 64) * shares + (int)blockIdx.z) * 64 + e % 64;
-      place[e] = at >= last ? -1 : order ? order[at] : at;
+      place[e] = at >= last || (!rows.starts && adapter_of(rows, at) != a) ? -1 : (int)row_at(rows, at);
     }
     __syncthreads();
     auto load = [&](int i, int buf) {
@@ -732,7 +731,7 @@ __global__ void __launch_bounds__(256) gather_mma_kernel(const GatherSide one, c
       for (int e = 0; e < 2; ++e) {
         const int c = c0 + warp * 16 + 8 * e + 2 * t;
         if (c < cols)
-          *reinterpret_cast<float2*>(side.part + (((int64_t)blockIdx.z * n_adapters + a) * rank + j) * cols + c) = make_float2(acc[m][e][2 * r], acc[m][e][2 * r + 1]);
+          *reinterpret_cast<float2*>(side.part + (((int64_t)blockIdx.z * rows.n + a) * rank + j) * cols + c) = make_float2(acc[m][e][2 * r], acc[m][e][2 * r + 1]);
       }
     }
 }
@@ -866,11 +865,10 @@ int tdb_lora_umma_gather(const Lora* l, const LoraGradients* g, void* stream) {
   };
   const GatherSide a = side(l->x, l->x_stride, l->cols, g->u, g->part_a, g->shares_a), b = side(l->dy, l->dy_stride, l->features, g->h, g->part_b, g->shares_b);
   const int r16 = r16_of(*l), mt = tdb_lora_umma_gather_factors(l) / 16, j_blocks = (r16 + 16 * mt - 1) / (16 * mt);
-  const LoraRows rows = lora_rows(*l);
   auto run = [&](auto kernel) {
     if (const int rc = opt_in_smem(reinterpret_cast<const void*>(kernel), gather_smem(mt))) return rc;
     kernel<<<dim3(a.blocks + b.blocks, l->n * j_blocks, std::max(a.shares, b.shares)), 256, gather_smem(mt), (cudaStream_t)stream>>>(
-        a, b, r16, l->rank, rows.order, rows.starts, (int)l->rows, l->n, j_blocks);
+        a, b, r16, l->rank, lora_rows(*l), j_blocks);
     return cuda_fail(cudaGetLastError(), "lora gather launch");
   };
   return mt == 1 ? run(gather_mma_kernel<1>) : mt == 2 ? run(gather_mma_kernel<2>) : run(gather_mma_kernel<4>);

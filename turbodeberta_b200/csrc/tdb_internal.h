@@ -216,8 +216,8 @@ TDB_HOST_API int tdb_lora_gather(const tdb::Lora* l, const tdb::LoraGradients* g
 TDB_HOST_API int tdb_lora_gather_sum(const tdb::Lora* l, const tdb::LoraGradients* g, void* stream);
 // The same on the tensor cores (lora_umma.cu), for bf16 with columns and features that are multiples of eight, all tensors 16-byte aligned and rows no
 // less than a row apart.  f: the factors that are multiplied with x (a) or dy (b turned, [n, rank, features]) in `shrink`, and those that make y (b) or dx (a
-// turned, [n, cols, rank]) in `product`.  hx, u, h: bf16 [rows, tdb_lora_inner()].  status: int32[4], word 0 tells of a wait that gave up.  `gather` goes by l->plan wherever the rows have ids; they lie in
-// the order of the rows.
+// turned, [n, cols, rank]) in `product`.  hx, u, h: bf16 [rows, tdb_lora_inner()].  status: int32[4], word 0 tells of a wait that gave up.  They lie in the order of the rows, with a
+// plan too.
 TDB_HOST_API int tdb_lora_umma_applies(const tdb::Lora* l);
 TDB_HOST_API int64_t tdb_lora_inner(const tdb::Lora* l);
 TDB_HOST_API int tdb_lora_umma_shrink(const tdb::Lora* l, int back, const void* f, void* hx, void* stream);

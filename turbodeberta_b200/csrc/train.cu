@@ -3,7 +3,8 @@
 // its outputs once, and what can be made again is not stored: the mask (philox.cuh) and the sum in front of the norm.
 //
 // Everything works on units of eight consecutive columns: a 16-byte load in bf16, two in fp32, and one block of random bits.
-// VEC: the rows allow that (columns a multiple of eight, aligned rows); otherwise a unit is read element by element.
+// VEC: the rows allow that (columns a multiple of eight, aligned rows); otherwise a unit is read element by element, and unless its elements share
+// random bits they are not neighbours but as far apart as there are units, so that the threads' loads are.
 #include "tdb_internal.h"
 #include "ptx_sm100.cuh"
 #include "philox.cuh"
@@ -21,7 +22,7 @@ __device__ __forceinline__ void to_type(__nv_bfloat16* p, float v) { *p = __floa
 template <typename T> struct Unit { uint4 v[sizeof(T) / 2]; };
 
 template <typename T, bool VEC>
-__device__ __forceinline__ Unit<T> load_unit(const T* p, int have) {
+__device__ __forceinline__ Unit<T> load_unit(const T* p, int have, int step = 1) {
   Unit<T> u;
   if (VEC) {
 #pragma unroll
@@ -29,7 +30,7 @@ __device__ __forceinline__ Unit<T> load_unit(const T* p, int have) {
   } else {
     T* e = reinterpret_cast<T*>(&u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { if (i < have) e[i] = p[i]; else to_type(e + i, 0.f); }
+    for (int i = 0; i < 8; ++i) { if (i < have) e[i] = p[i * step]; else to_type(e + i, 0.f); }
   }
   return u;
 }
@@ -67,7 +68,7 @@ __device__ __forceinline__ Eight eight(const Unit<__nv_bfloat16>& u) {
   return e;
 }
 template <bool VEC>
-__device__ __forceinline__ void store_unit(float* p, const Eight& x, int have) {
+__device__ __forceinline__ void store_unit(float* p, const Eight& x, int have, int step = 1) {
   float f[8];
   x.unpack(f);
   if (VEC) {
@@ -76,24 +77,25 @@ __device__ __forceinline__ void store_unit(float* p, const Eight& x, int have) {
       reinterpret_cast<uint4*>(p)[i] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < have) p[i] = f[i];
+    for (int i = 0; i < 8; ++i) if (i < have) p[i * step] = f[i];
   }
 }
 template <bool VEC>
-__device__ __forceinline__ void store_unit(__nv_bfloat16* p, const Eight& x, int have) {
+__device__ __forceinline__ void store_unit(__nv_bfloat16* p, const Eight& x, int have, int step = 1) {
   float f[8];
   x.unpack(f);
   if (VEC) {
     *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < have) p[i] = __float2bfloat16_rn(f[i]);
+    for (int i = 0; i < 8; ++i) if (i < have) p[i * step] = __float2bfloat16_rn(f[i]);
   }
 }
 // Eight weights of either type.
 template <bool VEC>
-__device__ __forceinline__ Eight load_weights(const void* w, int f32, int at, int have) {
-  return f32 ? eight(load_unit<float, VEC>(static_cast<const float*>(w) + at, have)) : eight(load_unit<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(w) + at, have));
+__device__ __forceinline__ Eight load_weights(const void* w, int f32, int at, int have, int step) {
+  return f32 ? eight(load_unit<float, VEC>(static_cast<const float*>(w) + at, have, step))
+             : eight(load_unit<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(w) + at, have, step));
 }
 __device__ __forceinline__ void drop8(Eight& x, const uint4& bits, uint32_t above, float scale) {
   float f[8];
@@ -164,10 +166,13 @@ __device__ __forceinline__ void warp_sums(float* v) {
     for (int off = 16; off >= 1; off >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
   }
 }
-template <int N>
+// A warp each, the whole block, or a part of the block with a barrier of its own: those come to sixteen barriers a block, of the 64 that an
+// SM has, which would leave it four blocks.
+enum { A_WARP, THE_BLOCK, A_PART };
+template <int N, int KIND = A_PART>
 __device__ __forceinline__ void group_sum(Group& g, float* v) {
   warp_sums<N>(v);
-  if (g.threads == 32) return;
+  if (KIND == A_WARP || g.threads == 32) return;
   const int warps = g.threads / 32;
   // two buffers in turn: a warp that runs ahead writes the other one, and cannot come round again before the next barrier
   float* buf = g.shared + (g.index * 2 + g.flip) * N * warps;
@@ -176,7 +181,8 @@ __device__ __forceinline__ void group_sum(Group& g, float* v) {
 #pragma unroll
     for (int i = 0; i < N; ++i) buf[g.lane / 32 * N + i] = v[i];
   }
-  asm volatile("bar.sync %0, %1;" ::"r"(g.index + 1), "r"(g.threads) : "memory");
+  if (KIND == THE_BLOCK) __syncthreads();
+  else asm volatile("bar.sync %0, %1;" ::"r"(g.index + 1), "r"(g.threads) : "memory");
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = 0.f;
 #pragma unroll 4
@@ -192,6 +198,15 @@ enum { ALONE = 0, JOIN = 1, JOIN_DROP = 2 };
 struct NormParams : Norm {
   int group, w_f32;                                         // threads of a row
 };
+
+// Which columns unit c is: the first, how far apart, and how many there are.
+struct Columns { int first, step, have; };
+template <bool VEC, int MODE>
+__device__ __forceinline__ Columns columns(int c, int units, int cols) {
+  if (VEC) return {c * 8, 1, 8};
+  if (MODE == JOIN_DROP) return {c * 8, 1, cols - c * 8};
+  return {c, units, (cols - c + units - 1) / units};
+}
 
 // Eight elements of what the norm is taken of; `bits` are those that dropped them.
 template <typename T, bool VEC, int MODE>
@@ -219,7 +234,7 @@ __device__ __forceinline__ void cut(Eight& x, int have) {
 
 // One group of threads to a row, the row in registers; mean first, then the deviations from it (the sum of squares alone would lose
 // the variance of rows far from zero).
-template <typename T, bool VEC, int MODE, int U>
+template <typename T, bool VEC, int MODE, int U, int KIND>
 __global__ void __launch_bounds__(512) norm_forward_kernel(const NormParams p) {
   extern __shared__ __align__(16) float shared[];
   Group g{p.group, (int)threadIdx.x % p.group, (int)threadIdx.x / p.group, shared, 0};
@@ -234,8 +249,9 @@ __global__ void __launch_bounds__(512) norm_forward_kernel(const NormParams p) {
   for (int i = 0; i < U; ++i) {
     const int c = g.lane + p.group * i;
     if (c < units) {
-      xu[i] = load_unit<T, VEC>(x + c * 8, p.cols - c * 8);
-      if (MODE != ALONE) ru[i] = load_unit<T, VEC>(res + c * 8, p.cols - c * 8);
+      const Columns at = columns<VEC, MODE>(c, units, p.cols);
+      xu[i] = load_unit<T, VEC>(x + at.first, at.have, at.step);
+      if (MODE != ALONE) ru[i] = load_unit<T, VEC>(res + at.first, at.have, at.step);
     }
   }
   Eight f[U];
@@ -251,7 +267,7 @@ __global__ void __launch_bounds__(512) norm_forward_kernel(const NormParams p) {
     }
   }
   float sum = halves(sums).x + halves(sums).y;
-  group_sum<1>(g, &sum);
+  group_sum<1, KIND>(g, &sum);
   const f32x2 mean = twice(sum / (float)p.cols), minus = twice(-halves(mean).x);
   f32x2 squares = twice(0.f);
 #pragma unroll
@@ -260,13 +276,13 @@ __global__ void __launch_bounds__(512) norm_forward_kernel(const NormParams p) {
     if (c < units) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) add2(f[i].v[e], minus);
-      if (!VEC) cut(f[i], p.cols - c * 8);
+      if (!VEC) cut(f[i], columns<VEC, MODE>(c, units, p.cols).have);
 #pragma unroll
       for (int e = 0; e < 4; ++e) fma2(squares, f[i].v[e], f[i].v[e]);
     }
   }
   float sq = halves(squares).x + halves(squares).y;
-  group_sum<1>(g, &sq);
+  group_sum<1, KIND>(g, &sq);
   const float inv = rsqrtf(sq / (float)p.cols + p.eps);
   if (p.stats && g.lane == 0) *reinterpret_cast<float2*>(p.stats + 2 * row) = make_float2(halves(mean).x, inv);
   const f32x2 scale = twice(inv);
@@ -274,10 +290,12 @@ __global__ void __launch_bounds__(512) norm_forward_kernel(const NormParams p) {
   for (int i = 0; i < U; ++i) {
     const int c = g.lane + p.group * i;
     if (c < units) {
-      const Eight w = load_weights<VEC>(p.w, p.w_f32, c * 8, p.cols - c * 8), b = load_weights<VEC>(p.b, p.w_f32, c * 8, p.cols - c * 8);
+      const Columns at = columns<VEC, MODE>(c, units, p.cols);
+      const Eight w = load_weights<VEC>(p.w, p.w_f32, at.first, at.have, at.step);
+      const Eight b = load_weights<VEC>(p.b, p.w_f32, at.first, at.have, at.step);
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[i].v[e] = fused(times(f[i].v[e], scale), w.v[e], b.v[e]);
-      store_unit<VEC>((T*)p.y + row * p.cols + c * 8, f[i], p.cols - c * 8);
+      store_unit<VEC>((T*)p.y + row * p.cols + at.first, f[i], at.have, at.step);
     }
   }
 }
@@ -310,13 +328,14 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormParams 
     const int c = g.lane + p.group * i;
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[i].v[e] = dw[i].v[e] = db[i].v[e] = twice(0.f);
-    if (c < units) w[i] = load_weights<VEC>(p.w, p.w_f32, c * 8, p.cols - c * 8);
+    const Columns at = columns<VEC, MODE>(c, units, p.cols);
+    if (c < units) w[i] = load_weights<VEC>(p.w, p.w_f32, at.first, at.have, at.step);
   }
   const float over = 1.f / (float)p.cols;
   const int64_t first = ((int64_t)blockIdx.x * groups + g.index) * R, stride = (int64_t)gridDim.x * groups * R;
   // tensor k of x, residual, dy
-  auto source = [&](int k, int64_t row, int c) {
-    return k == 0 ? (const T*)p.x + row * p.x_stride + c * 8 : k == NT - 1 ? (const T*)p.dy + row * p.dy_stride + c * 8 : (const T*)p.res + row * p.res_stride + c * 8;
+  auto source = [&](int k, int64_t row, int col) {
+    return k == 0 ? (const T*)p.x + row * p.x_stride + col : k == NT - 1 ? (const T*)p.dy + row * p.dy_stride + col : (const T*)p.res + row * p.res_stride + col;
   };
   const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16, pitch = blockDim.x * 16;
   const uint32_t stage_bytes = NT * R * U * PIECES * pitch;
@@ -327,7 +346,7 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormParams 
       if (row0 + r >= p.rows) break;
 #pragma unroll
       for (int k = 0; k < NT; ++k) {
-        const T* row = source(k, row0 + r, g.lane);
+        const T* row = source(k, row0 + r, g.lane * 8);
 #pragma unroll
         for (int i = 0; i < U; ++i)
           if (g.lane + p.group * i < units) {
@@ -350,7 +369,8 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormParams 
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(slot(stage, k, r, i, piece)) : "memory");
       }
     } else {
-      u = load_unit<T, false>(source(k, row, c), p.cols - c * 8);
+      const Columns at = columns<VEC, MODE>(c, units, p.cols);
+      u = load_unit<T, false>(source(k, row, at.first), at.have, at.step);
     }
     return u;
   };
@@ -389,7 +409,7 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormParams 
         const Eight d = eight(unit(stage, NT - 1, row0 + r, r, i));          // zeros behind the last column, and in w too
 #pragma unroll
         for (int e = 0; e < 4; ++e) h[r][i].v[e] = times(plus(h[r][i].v[e], minus), inv);
-        if (!VEC) cut(h[r][i], p.cols - c * 8);
+        if (!VEC) cut(h[r][i], columns<VEC, MODE>(c, units, p.cols).have);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           fma2(dw[i].v[e], d.v[e], h[r][i].v[e]);
@@ -415,12 +435,13 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormParams 
         Eight d = eight(unit(stage, NT - 1, row, r, i));
 #pragma unroll
         for (int e = 0; e < 4; ++e) d.v[e] = times(fused(h[r][i].v[e], c2, fused(d.v[e], w[i].v[e], c1)), inv);
-        const int64_t at = row * p.cols + c * 8;
-        if (MODE == ALONE && p.dx) store_unit<VEC>((T*)p.dx + at, d, p.cols - c * 8);
-        if (MODE != ALONE && p.dres) store_unit<VEC>((T*)p.dres + at, d, p.cols - c * 8);
+        const Columns to = columns<VEC, MODE>(c, units, p.cols);
+        const int64_t at = row * p.cols + to.first;
+        if (MODE == ALONE && p.dx) store_unit<VEC>((T*)p.dx + at, d, to.have, to.step);
+        if (MODE != ALONE && p.dres) store_unit<VEC>((T*)p.dres + at, d, to.have, to.step);
         if (MODE == JOIN_DROP && p.dx) {
           drop8(d, bits[r][i], above, p.drop.scale);
-          store_unit<VEC>((T*)p.dx + at, d, p.cols - c * 8);
+          store_unit<VEC>((T*)p.dx + at, d, to.have, to.step);
         }
       }
     }
@@ -451,7 +472,7 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormParams 
   }
   __syncthreads();
   for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
-    const int at = (c & 7) * units + (c >> 3);
+    const int at = VEC || MODE == JOIN_DROP ? (c & 7) * units + (c >> 3) : c;
     p.partial[(int64_t)blockIdx.x * 2 * p.cols + c] = sum[at];
     p.partial[((int64_t)blockIdx.x * 2 + 1) * p.cols + c] = sum[8 * units + at];
   }
@@ -488,15 +509,16 @@ int norm_forward(NormParams p, cudaStream_t s) {
   if (const int rc = device_sms(&sms)) return rc;
   auto run = [&](auto kernel, int u) {
     p.group = group_threads(units, u);
-    const int groups = p.rows >= 16 * sms ? max(1, 256 / p.group) : 1;      // few rows: one per block, so that they spread over the SMs
+    const int groups = p.group == 32 && p.rows >= 16 * sms ? 8 : 1;       // few rows: one to a block, so that they spread over the SMs
     const int64_t blocks = (p.rows + groups - 1) / groups;
-    kernel<<<(unsigned)blocks, groups * p.group, p.group == 32 ? 0 : groups * 2 * (p.group / 32) * sizeof(float), s>>>(p);
+    kernel<<<(unsigned)blocks, groups * p.group, p.group == 32 ? 0 : 2 * (p.group / 32) * sizeof(float), s>>>(p);
     return cuda_fail(cudaGetLastError(), "norm launch");
   };
-  if (units <= 32) return run(norm_forward_kernel<T, VEC, MODE, 1>, 1);
-  if (units <= 64) return run(norm_forward_kernel<T, VEC, MODE, 2>, 2);
-  if (units <= 96) return run(norm_forward_kernel<T, VEC, MODE, 3>, 3);
-  return run(norm_forward_kernel<T, VEC, MODE, 4>, 4);
+  if (units <= 32) return run(norm_forward_kernel<T, VEC, MODE, 1, A_WARP>, 1);
+  if (units <= 64) return run(norm_forward_kernel<T, VEC, MODE, 2, A_WARP>, 2);
+  if (units <= 96) return run(norm_forward_kernel<T, VEC, MODE, 3, A_WARP>, 3);
+  if (units <= 128) return run(norm_forward_kernel<T, VEC, MODE, 4, A_WARP>, 4);
+  return run(norm_forward_kernel<T, VEC, MODE, 4, THE_BLOCK>, 4);
 }
 
 struct BackwardShape { int units_each, rows_each, group, groups, blocks; };
