@@ -105,28 +105,32 @@ __device__ __forceinline__ void drop8(Eight& x, const uint4& bits, uint32_t abov
 }
 
 // ------------------------------------------------------------------------------------------------------------------ dropout
-// y = what stays of x, scaled; its backward pass is the same of dy.  PER units to a thread, all loaded before the first is used.
+// y = what stays of x, scaled; its backward pass is the same of dy.  PER units to a thread, all loaded before the first is used.  16384 x 1024 bf16: bound by
+// the generator's instructions (154 for eight elements, 69 % of the issue slots) before memory.
 template <typename T, bool VEC, int PER>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, T* __restrict__ y, int64_t n, Dropout key) {
-  const int64_t units = (n + 7) / 8, first = ((int64_t)blockIdx.x * 256 * PER) + threadIdx.x;
+  const int64_t full = VEC ? n / 8 : 0, first = (int64_t)blockIdx.x * 256 * PER + threadIdx.x;
   const uint64_t seed = dropout_seed(key);
-  Unit<T> u[PER];
+  const uint32_t above = dropout_above(key.drop);
+  auto drop = [&](const Unit<T>& u, int64_t at) {
+    Eight f = eight(u);
+    drop8(f, philox((uint64_t)at, (uint64_t)key.offset, seed), above, key.scale);
+    return f;
+  };
+  if (VEC && ((int64_t)blockIdx.x + 1) * 256 * PER <= full) {        // every unit of the block is a whole one
+    Unit<T> u[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int64_t at = first + 256 * i;
-    if (at >= units) break;
-    const int have = (int)min((int64_t)8, n - at * 8);
-    u[i] = VEC && have == 8 ? load_unit<T, true>(x + at * 8, 8) : load_unit<T, false>(x + at * 8, have);
+    for (int i = 0; i < PER; ++i) u[i] = load_unit<T, true>(x + (first + 256 * i) * 8, 8);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) store_unit<true>(y + (first + 256 * i) * 8, drop(u[i], first + 256 * i), 8);
+    return;
   }
-#pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int64_t at = first + 256 * i;
-    if (at >= units) break;
+    if (at * 8 >= n) return;
     const int have = (int)min((int64_t)8, n - at * 8);
-    Eight f = eight(u[i]);
-    drop8(f, philox((uint64_t)at, (uint64_t)key.offset, seed), dropout_above(key.drop), key.scale);
-    if (VEC && have == 8) store_unit<true>(y + at * 8, f, 8);
-    else store_unit<false>(y + at * 8, f, have);
+    if (at < full) store_unit<true>(y + at * 8, drop(load_unit<T, true>(x + at * 8, 8), at), 8);
+    else store_unit<false>(y + at * 8, drop(load_unit<T, false>(x + at * 8, have), at), have);
   }
 }
 
