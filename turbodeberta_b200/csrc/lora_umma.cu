@@ -2,8 +2,8 @@
 //
 // Going forward: `shrink` makes the inner values h = s x A^T of every row, then one tcgen05 product makes y, bias and adapters included.
 // The adapters' part is a few more columns of the product's inner dimension: behind the tiles of x and W come tiles of h and B_a, and the
-// accumulator never leaves tensor memory in between.  A tile whose rows belong to D adapters takes D such steps, each with zeros in place
-// of the other adapters' rows.  Coming back the same kernel makes dx = dy W + u A, with W read along its other axis, and `gather` the
+// accumulator never leaves tensor memory in between.  A tile whose rows belong to several adapters takes the columns of each, one behind the other, with
+// zeros in the rows of the others.  Coming back the same kernel makes dx = dy W + u A, with W read along its other axis, and `gather` the
 // adapters' gradients.
 //
 // Inner values are held as the sum of two bf16 numbers (hi and lo, 2^-16 of the value or less away from it): rounding them to one would add an
@@ -226,26 +226,6 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ bool test_wait(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-  return ok != 0;
-}
-// mbar_wait() that polls.
-__device__ __forceinline__ bool polling_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code, uint64_t limit_ns) {
-  for (int i = 0; i < 64; ++i)
-    if (test_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  while (!*abort_flag) {
-    for (int i = 0; i < 64; ++i)
-      if (test_wait(bar, parity)) return true;
-    if (globaltimer_ns() - t0 > limit_ns) {
-      *abort_flag = 1;
-      if (*reinterpret_cast<volatile int*>(status) == 0) *reinterpret_cast<volatile int*>(status) = code;
-    }
-  }
-  return false;
-}
 template <int CTAS>
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1) {
   if (CTAS == 2)                                       // may signal the neighbour's barrier
@@ -340,7 +320,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
   volatile int* counted = reinterpret_cast<volatile int*>(gbase + BARS + 268);                 // tiles whose adapters have been counted
   volatile uint16_t* counts = reinterpret_cast<volatile uint16_t*>(gbase + BARS + 512);
   volatile uint32_t* bad_factors = reinterpret_cast<volatile uint32_t*>(gbase + BARS + 264);
-  auto wait = [&](int i, int phase) { return (CTAS == 2 ? polling_wait : mbar_wait)(bar(i), (uint32_t)(phase & 1), abort_flag, p.status, 200 + i, WAIT_NS); };
+  auto wait = [&](int i, int phase) { return mbar_wait(bar(i), (uint32_t)(phase & 1), abort_flag, p.status, 200 + i, WAIT_NS); };
   const uint32_t rank = CTAS == 2 ? cta_rank() : 0;
   auto first_cta = [&](uint32_t addr) { return CTAS == 2 ? in_cta(addr, 0) : addr; };
   if (tid == 0) {
@@ -376,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
         }
     }
     __threadfence_block();
-    return (int)counts[i];
+    return *counted > i ? (int)counts[i] : 0;          // none where a wait has given up: whoever else knows of some finds its waits over at once
   };
   auto tile_row = [&](int tile) { return (int64_t)(tile / n_tiles) * BM * CTAS; };
 
@@ -477,15 +457,15 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
 #pragma unroll
             for (int r = 0; r < 2; ++r)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) copy(place(r, four + i), mine[r] == a ? h + (int64_t)r * 64 * inner + q + 8 * i : p.hx, mine[r] == a);
+              for (int i = 0; i < 4; ++i) copy(place(r, four + i), mine[r] == a && a >= 0 ? h + (int64_t)r * 64 * inner + q + 8 * i : p.hx, mine[r] == a && a >= 0);
 #pragma unroll
             for (int r = 0; r < BR; ++r) {
               const int n = n0 + me + 64 * r;
-              const bf16* row = p.f + ((int64_t)a * p.N + min(n, p.N - 1)) * p.rank;
+              const bf16* row = p.f + ((int64_t)max(a, 0) * p.N + min(n, p.N - 1)) * p.rank;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int j = q + 8 * i >= p.r16 ? q + 8 * i - p.r16 : q + 8 * i;
-                const bool real = n < p.N && j < p.rank;
+                const bool real = a >= 0 && n < p.N && j < p.rank;
                 if (VEC) {
                   copy(place(r, four + i) + A_BYTES, real ? row + j : p.f, real);
                 } else {
@@ -636,8 +616,8 @@ __global__ void __launch_bounds__(THREADS, 1) lora_product_kernel(const __grid_c
 // ------------------------------------------------------------------------------------------------------------------- gather
 // part[z][a][j][c] = sum over a share of the rows t of adapter a of v[t][j] x[t][c], v being the sum of two bf16 numbers.  A block: one
 // adapter, 16 MT factors, 128 columns; a warp: 16 columns.  The adapter's rows, which the plan lists, come in tiles of 64 through shared memory, two at
-// a time; blockIdx.z takes every shares-th tile.  Without a plan (few rows) all rows do, zeros in the place of those that are not the adapter's.  Both gradients in one launch (blockIdx.x: the blocks of columns of the first, then those of the
-// second).  Bound by reading x.
+// a time; blockIdx.z takes every shares-th tile.  Without a plan (few rows) all rows do, zeros in the place of those that are not the adapter's.  Both
+// gradients in one launch (blockIdx.x: the blocks of columns of the first, then those of the second).  Bound by reading x.
 constexpr int GC = 128, GP = GC + 8, G_BATCH = 16;     // G_BATCH: tiles whose rows are looked up at once
 __host__ __device__ constexpr int gather_pitch(int mt) { return 32 * mt + 8; }
 __host__ __device__ constexpr int gather_smem(int mt) { return 2 * 64 * (GP + gather_pitch(mt)) * 2; }
