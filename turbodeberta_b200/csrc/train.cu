@@ -239,7 +239,7 @@ __device__ __forceinline__ void cut(Eight& x, int have) {
 // One group of threads to a row, the row in registers; mean first, then the deviations from it (the sum of squares alone would lose
 // the variance of rows far from zero).
 template <typename T, bool VEC, int MODE, int U, int KIND>
-__global__ void __launch_bounds__(512) norm_forward_kernel(const NormParams p) {
+__global__ void __launch_bounds__(KIND == A_WARP ? 256 : 512, KIND == A_WARP ? 4 : 1) norm_forward_kernel(const NormParams p) {
   extern __shared__ __align__(16) float shared[];
   Group g{p.group, (int)threadIdx.x % p.group, (int)threadIdx.x / p.group, shared, 0};
   const int groups = blockDim.x / p.group;
