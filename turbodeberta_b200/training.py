@@ -35,8 +35,10 @@ def _fresh_seed(x: torch.Tensor) -> torch.Tensor:
     return torch.empty((1,), dtype=torch.int64, device=x.device).random_()
 
 
-def _hooked(module: nn.Module) -> bool:
-    return bool(module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
+def _stock(module: nn.Module, types) -> bool:
+    """Whether one kernel may do what calling the module does: exactly one of ``types``, no subclass, with no ``forward`` of its own and no hooks."""
+    return (type(module) in types and "forward" not in module.__dict__
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
 
 
 class FlashLayerNorm(nn.LayerNorm):
@@ -59,9 +61,9 @@ class _JoinedEnd:
     def forward(self, hidden_states, input_tensor):
         x = self.dense(hidden_states)
         norm, drop = self.LayerNorm, self.dropout
-        if (isinstance(norm, nn.LayerNorm) and isinstance(drop, (nn.Dropout, nn.Identity)) and x.shape == input_tensor.shape
-                and x.dtype == input_tensor.dtype and _norm_applies(norm, x) and not _hooked(norm) and not _hooked(drop)):
-            p = drop.p if isinstance(drop, nn.Dropout) and drop.training else 0.0
+        if (_stock(norm, NORMS) and _stock(drop, (*DROPOUTS, nn.Identity)) and not nn.modules.module._has_any_global_hook()
+                and x.shape == input_tensor.shape and x.dtype == input_tensor.dtype and _norm_applies(norm, x)):
+            p = drop.p if type(drop) in DROPOUTS and drop.training else 0.0
             return dropout_add_layer_norm(x, input_tensor, norm.weight, norm.bias, norm.eps, p, _fresh_seed(x) if p > 0 else None)
         return norm(drop(x) + input_tensor)
 
