@@ -633,7 +633,7 @@ class FlashDebertaV2Model(DebertaV2Model):
 def patch_model(model: nn.Module, train_kernels: bool = False) -> nn.Module:
     """Swap, in place, every eager ``DisentangledSelfAttention`` of an already built HF DeBERTa-v2 model for
     the fused module (parameters are shared, not copied) and give its encoder the cached relative embeddings.
-    ``train_kernels``: passes that record gradients run their LayerNorms, dropouts and sublayer ends on this library's
+    ``train_kernels``: modules in training mode, and passes that record gradients, run their LayerNorms, dropouts and sublayer ends on this library's
     kernels too (``training.py``); dropout then draws other numbers than torch's for the same seed."""
     for name, mod in list(model.named_modules()):
         if isinstance(mod, DebertaV2Attention) and not isinstance(mod.self, FlashDisentangledSelfAttention):

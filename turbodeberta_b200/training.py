@@ -2,7 +2,9 @@
 
 ``patch_model(model, train_kernels=True)`` gives the stock modules these classes (parameters and names stay): LayerNorms and dropouts run the
 kernels of ``ops.layer_norm`` and ``ops.dropout``, and the ends of both halves of a layer (``DebertaV2SelfOutput``, ``DebertaV2Output``: dropout,
-residual, LayerNorm) run as one.  Passes without gradients, other types than float32 and bfloat16, autocast and the CPU run as before.
+residual, LayerNorm) run as one.  Passes of modules in eval mode that record no gradients, other types than float32 and bfloat16, autocast and the
+CPU run as before.  In training mode the kernels run without gradients too: a checkpoint's first pass may be one without, and the pass that is made
+again for its gradients has to drop the same elements.
 
 The attention has no backward pass (neither has the reference's), so a training loop reaches what lies behind the last attention whose
 inputs are frozen: task heads, and the last layer's projections, norms and adapters.
@@ -19,13 +21,13 @@ from .ops.layer_norm import dropout_add_layer_norm, layer_norm
 _TYPES = (torch.float32, torch.bfloat16)
 
 
-def _applies(x: torch.Tensor) -> bool:
-    return torch.is_grad_enabled() and x.is_cuda and x.dtype in _TYPES and not torch.is_autocast_enabled()
+def _applies(module: nn.Module, x: torch.Tensor) -> bool:
+    return (module.training or torch.is_grad_enabled()) and x.is_cuda and x.dtype in _TYPES and not torch.is_autocast_enabled()
 
 
 def _norm_applies(norm: nn.LayerNorm, x: torch.Tensor) -> bool:
     w, b = norm.weight, norm.bias
-    return (_applies(x) and w is not None and b is not None and w.dim() == 1 and w.dtype == b.dtype and w.dtype in (x.dtype, torch.float32)
+    return (_applies(norm, x) and w is not None and b is not None and w.dim() == 1 and w.dtype == b.dtype and w.dtype in (x.dtype, torch.float32)
             and x.shape[-1] == w.numel() and w.numel() <= 16384)
 
 
@@ -50,7 +52,7 @@ class FlashLayerNorm(nn.LayerNorm):
 
 class FlashDropout(nn.Dropout):
     def forward(self, x):
-        if self.training and self.p > 0 and not self.inplace and _applies(x):
+        if self.training and self.p > 0 and not self.inplace and _applies(self, x):
             return dropout(x, self.p, _fresh_seed(x))
         return super().forward(x)
 
