@@ -10,6 +10,10 @@
 
 One batch mixes requests of any adapters (``ops.lora.lora_linear``), on the padded and the packed route alike.  The reference has nothing of
 this kind; there every fine-tuning is a model of its own.
+
+The ids are those of the thread and of the block, and neither need be the same when a checkpointed pass is made again: that happens within the backward
+pass, in autograd's own thread.  ``checkpoint(keep_adapters(part), x, ...)``, or ``checkpoint(part, x, use_reentrant=False,
+context_fn=recompute_contexts)``, gives the pass its ids again; without either it raises.
 """
 from __future__ import annotations
 
@@ -28,14 +32,28 @@ DEFAULT_TARGETS = ("self.value_proj", "attention.output.dense", "intermediate.de
 class _Active(threading.local):
     ids = None                  # of the batch's sequences
     rows = None                 # of the packed stream's tokens
+    task = -1                   # the backward pass within which both were chosen; -1: none
 
 
 _ACTIVE = _Active()
+_backward_pass = torch._C._current_graph_task_id             # that this thread is running; -1: none
+
+
+@contextlib.contextmanager
+def _active(ids, rows):
+    before = (_ACTIVE.ids, _ACTIVE.rows, _ACTIVE.task)
+    _ACTIVE.ids, _ACTIVE.rows, _ACTIVE.task = ids, rows, _backward_pass()
+    try:
+        yield
+    finally:
+        _ACTIVE.ids, _ACTIVE.rows, _ACTIVE.task = before
 
 
 class AdapterLinear(nn.Module):
     """A frozen ``nn.Linear`` with ``count`` adapters of up to ``rank``: ``lora_a [count, rank, in]`` (small random numbers) and ``lora_b [count, out,
     rank]`` (zeros, so that a fresh adapter changes nothing).  Outside ``use_adapters`` it is the Linear alone."""
+
+    _used = False               # with ids, ever
 
     def __init__(self, base: nn.Linear, count: int, rank: int, scaling: float = 1.0):
         super().__init__()
@@ -50,8 +68,12 @@ class AdapterLinear(nn.Module):
 
     def forward(self, x):
         ids = _ACTIVE.ids if _ACTIVE.rows is None else _ACTIVE.rows
+        if self._used and _ACTIVE.task != _backward_pass():  # made again by a checkpoint: what is in use here, if anything, need not be the first pass's
+            raise RuntimeError("a checkpointed pass is being made again and does not know its adapter ids: checkpoint keep_adapters(function), or give "
+                               "checkpoint context_fn=recompute_contexts")
         if ids is None:
             return self.base(x)
+        self._used = True
         if ids.device != x.device:
             ids = ids.to(x.device)
         return lora_linear(x, self.base.weight, self.base.bias, self.lora_a, self.lora_b, self.scaling, ids)
@@ -122,12 +144,25 @@ def use_adapters(ids):
         raise ValueError("ids must be one integer for each sequence of the batch")
     if not ids.is_cuda and torch.cuda.is_available():
         ids = ids.cuda()
-    before = (_ACTIVE.ids, _ACTIVE.rows)
-    _ACTIVE.ids, _ACTIVE.rows = ids, None
-    try:
+    with _active(ids, None):
         yield
-    finally:
-        _ACTIVE.ids, _ACTIVE.rows = before
+
+
+def keep_adapters(function):
+    """``function``, called with the adapter ids (or none) that are in use now, whichever thread calls it and whenever: what a checkpoint is to be given."""
+    ids, rows = _ACTIVE.ids, _ACTIVE.rows
+
+    def kept(*args, **kwargs):
+        with _active(ids, rows):
+            return function(*args, **kwargs)
+
+    return kept
+
+
+def recompute_contexts():
+    """The ``context_fn`` of a checkpoint without ``use_reentrant``: the pass that is made again has the ids of the first.  In a Hugging Face model:
+    ``model.gradient_checkpointing_enable({"use_reentrant": False, "context_fn": recompute_contexts})``."""
+    return contextlib.nullcontext(), _active(_ACTIVE.ids, _ACTIVE.rows)
 
 
 @contextlib.contextmanager
