@@ -296,11 +296,10 @@ Tensor lora_shrink(const LoraCall& c, bool back, const Tensor& f, cudaStream_t s
   }
   return h;
 }
-// y [rows, features], or dx [rows, cols], from the rows and their inner values.
-Tensor lora_product(const LoraCall& c, bool back, const Tensor& f, const Tensor& h, c10::cuda::CUDAStream stream) {
-  const int64_t cols = back ? c.l.cols : c.l.features;
+// y or dx, in `shape`, from the rows and their inner values.  Never a view: autograd would let nobody change a node's output in place.
+Tensor lora_product(const LoraCall& c, bool back, const Tensor& f, const Tensor& h, at::IntArrayRef shape, c10::cuda::CUDAStream stream) {
   if (c.tensor_cores) {
-    Tensor y = at::empty({c.l.rows, cols}, c.w.options());
+    Tensor y = at::empty(shape, c.w.options());
     if (!back && tdb_lora_skinny_applies(&c.l)) {
       check_rc(tdb_lora_skinny(&c.l, h.data_ptr(), y.data_ptr(), stream.stream()));
       return y;
@@ -311,7 +310,7 @@ Tensor lora_product(const LoraCall& c, bool back, const Tensor& f, const Tensor&
     return y;
   }
   const Tensor base = back ? c.product(c.dy.t, c.w) : c.product(c.x.t, c.w.t());
-  Tensor y = c.l.dtype == TDB_DTYPE_F32 ? base : at::empty({c.l.rows, cols}, c.w.options());
+  Tensor y = c.l.dtype == TDB_DTYPE_F32 ? at::_unsafe_view(base, shape) : at::empty(shape, c.w.options());
   check_rc(tdb_lora_expand(&c.l, back, base.data_ptr<float>(), h.data_ptr<float>(), y.data_ptr(), stream.stream()));
   return y;
 }
@@ -327,7 +326,7 @@ std::tuple<Tensor, Tensor, Tensor> run_lora(LoraCall& c, at::IntArrayRef shape, 
     c.l.plan = plan.data_ptr<int32_t>();
   }
   const Tensor h = lora_shrink(c, false, c.a, stream);
-  return {lora_product(c, false, c.b, h, stream).view(shape), h, plan};
+  return {lora_product(c, false, c.b, h, shape, stream), h, plan};
 }
 
 // (gradient of a, gradient of b), where u and h are given.
@@ -385,7 +384,7 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
       }
       // the product may start beside the kernel in front of it, which therefore is the one that makes u
       u = lora_shrink(c, true, b_turned, stream);
-      if (need_x) dx = lora_product(c, true, a_turned, u, stream).view(x.sizes());
+      if (need_x) dx = lora_product(c, true, a_turned, u, x.sizes(), stream);
     }
     if (c.l.rows == 0) {
       if (need_a) da = at::zeros_like(a);
