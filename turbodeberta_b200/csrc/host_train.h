@@ -29,6 +29,12 @@ void refuse_second_derivative(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "turbodeberta_b200: ", what, " has no second derivative (create_graph=True)");
 }
 
+// A tangent (torch.autograd.forward_ad) would be lost without a word: it is no reason for autograd to record a node.  Undefined tensors have none.
+void refuse_tangents(const char* what, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(!t || !t->_fw_grad(0).defined(), "turbodeberta_b200: ", what, " has no forward-mode derivative");
+}
+
 void check_probability(double p) {
   if (!(p >= 0.0 && p <= 1.0)) throw py::value_error("dropout probability has to be between 0 and 1, but got " + std::to_string(p));
 }
@@ -69,6 +75,7 @@ class DropoutNode : public torch::autograd::Function<DropoutNode> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dy) {
     refuse_second_derivative("dropout");
+    refuse_tangents("dropout", {&dy[0]});
     const Tensor seed = ctx->get_saved_variables()[0];
     const auto d = dropout_of(ctx->saved_data["p"].toDouble(), seed.defined() ? OptTensor(seed) : std::nullopt, ctx->saved_data["value"].toInt(),
                               ctx->saved_data["offset"].toInt());
@@ -81,6 +88,7 @@ Tensor dropout(const Tensor& x, double p, const OptTensor& seed, int64_t seed_va
   check_probability(p);
   check_seed(seed, x);
   device_of({&x});
+  refuse_tangents("dropout", {&x});
   const auto d = dropout_of(p, seed, seed_value, offset);
   if (at::GradMode::is_enabled() && x.requires_grad()) return DropoutNode::apply(x, seed, seed_value, offset, p);
   return run_dropout(x, d);
@@ -129,6 +137,7 @@ class NormNode : public torch::autograd::Function<NormNode> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     refuse_second_derivative("layer_norm");
+    refuse_tangents("layer_norm", {&grads[0]});
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &res = saved[1], &w = saved[2], &stats = saved[3], &seed = saved[4];
     const bool need_x = ctx->needs_input_grad(0), need_res = res.defined() && ctx->needs_input_grad(1);
@@ -187,6 +196,7 @@ Tensor norm(const Tensor& x, const OptTensor& res, const Tensor& w, const Tensor
   check_probability(p);
   check_seed(seed, x);
   device_of({&x, res ? &*res : nullptr, &w, &b});
+  refuse_tangents("layer_norm", {&x, res ? &*res : nullptr, &w, &b});
   const auto d = dropout_of(p, seed, seed_value, offset);
   if (at::GradMode::is_enabled() && (x.requires_grad() || (res && res->requires_grad()) || w.requires_grad() || b.requires_grad()))
     return NormNode::apply(x, res, w, b, eps, p, seed, seed_value, offset);
@@ -360,6 +370,7 @@ class LoraNode : public torch::autograd::Function<LoraNode> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     refuse_second_derivative("lora_linear");
+    refuse_tangents("lora_linear", {&grads[0]});
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &a = saved[2], &b = saved[3], &scaling = saved[4], &ids = saved[5], &h = saved[6], &plan = saved[7];
     const int at = ctx->saved_data["bias"].toBool() ? 3 : 2;
@@ -421,6 +432,7 @@ Tensor lora_linear(const Tensor& x, const Tensor& w, const OptTensor& bias, cons
     if (!rows && !first) throw py::value_error("adapter_ids must have the shape of x without its last dimension, or one entry for each entry of x's first");
   }
   device_of({&x, &w, bias ? &*bias : nullptr, &a, &b, scaling ? &*scaling : nullptr, ids ? &*ids : nullptr});
+  refuse_tangents("lora_linear", {&x, &w, bias ? &*bias : nullptr, &a, &b, scaling ? &*scaling : nullptr});
   std::vector<int64_t> shape = x.sizes().vec();
   shape.back() = N;
   if (at::GradMode::is_enabled()) {

@@ -29,7 +29,8 @@ def signed64(value, name: str) -> int:
 
 
 def dropout(x: torch.Tensor, p: float, seed, offset: int = 0) -> torch.Tensor:
-    """Drop elements of ``x`` (float32 or bfloat16, any shape and strides) with probability ``p``; differentiable in ``x``.
+    """Drop elements of ``x`` (float32 or bfloat16, any shape and strides) with probability ``p``; differentiable in ``x`` (once, and
+    backward: a second derivative and forward-mode tangents are refused).
 
     ``seed`` is a number, or an int64 CUDA tensor of one element that the kernels read: in a CUDA graph a number is recorded with the
     launch, so every replay drops the same elements, while a tensor may be given new values between replays (a forward pass and its

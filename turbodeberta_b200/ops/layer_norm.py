@@ -5,6 +5,7 @@
 ``DebertaV2SelfOutput`` and ``DebertaV2Output`` of the HF model end in.  Sums, means and deviations are taken in fp32 and the result is
 rounded once; the backward pass makes the dropout mask and the sum again from ``x`` and ``residual``.  Gradients of the weights are added
 up in a fixed order: two runs give the same bits.
+Second derivatives and forward-mode tangents are refused.
 """
 from __future__ import annotations
 

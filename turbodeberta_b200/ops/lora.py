@@ -2,7 +2,7 @@
 
 ``y[t] = x[t] W^T + b + s_a (x[t] A_a^T) B_a^T`` with ``a`` the adapter of row ``t``: one model's projection serves fine-tunings of many
 owners in one batch, each row with its own.  Rows may come in any order and an adapter may appear in any number of places.  Differentiable
-in ``x``, ``lora_a`` and ``lora_b``; the shared projection is frozen.
+in ``x``, ``lora_a`` and ``lora_b`` (once, and backward: a second derivative and forward-mode tangents are refused); the shared projection is frozen.
 """
 from __future__ import annotations
 

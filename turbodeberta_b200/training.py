@@ -2,8 +2,8 @@
 
 ``patch_model(model, train_kernels=True)`` gives the stock modules these classes (parameters and names stay): LayerNorms and dropouts run the
 kernels of ``ops.layer_norm`` and ``ops.dropout``, and the ends of both halves of a layer (``DebertaV2SelfOutput``, ``DebertaV2Output``: dropout,
-residual, LayerNorm) run as one.  Passes of modules in eval mode that record no gradients, other types than float32 and bfloat16, autocast and the
-CPU run as before.  In training mode the kernels run without gradients too: a checkpoint's first pass may be one without, and the pass that is made
+residual, LayerNorm) run as one.  Passes of modules in eval mode that record no gradients, other types than float32 and bfloat16, autocast, forward-mode
+derivatives, ``torch.func``'s transforms and the CPU run as before.  In training mode the kernels run without gradients too: a checkpoint's first pass may be one without, and the pass that is made
 again for its gradients has to drop the same elements.
 
 The attention has no backward pass (neither has the reference's), so a training loop reaches what lies behind the last attention whose
@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 from transformers.models.deberta_v2.modeling_deberta_v2 import DebertaV2Output, DebertaV2SelfOutput
 
 from .ops.dropout import dropout
@@ -22,7 +23,8 @@ _TYPES = (torch.float32, torch.bfloat16)
 
 
 def _applies(module: nn.Module, x: torch.Tensor) -> bool:
-    return (module.training or torch.is_grad_enabled()) and x.is_cuda and x.dtype in _TYPES and not torch.is_autocast_enabled()
+    return ((module.training or torch.is_grad_enabled()) and x.is_cuda and x.dtype in _TYPES and not torch.is_autocast_enabled()
+            and forward_ad._current_level < 0 and torch._C._functorch.peek_interpreter_stack() is None)
 
 
 def _norm_applies(norm: nn.LayerNorm, x: torch.Tensor) -> bool:
