@@ -76,7 +76,13 @@ class AdapterLinear(nn.Module):
         self._used = True
         if ids.device != x.device:
             ids = ids.to(x.device)
-        return lora_linear(x, self.base.weight, self.base.bias, self.lora_a, self.lora_b, self.scaling, ids)
+        inputs = [x, self.base.weight, self.base.bias, self.lora_a, self.lora_b]
+        if not torch.is_autocast_enabled(x.device.type):
+            return lora_linear(*inputs, self.scaling, ids)
+        # as an nn.Linear: operands of any type but fp64, the result in autocast's.  The kernels have no fp16: its operands are computed in fp32.
+        to = torch.get_autocast_dtype(x.device.type)
+        inputs = [t if t is None or t.dtype == torch.float64 else t.to(to).to(torch.bfloat16 if to == torch.bfloat16 else torch.float32) for t in inputs]
+        return lora_linear(*inputs, self.scaling, ids).to(to)
 
     def extra_repr(self):
         return f"count={self.count}, rank={self.rank}, scaling={self.scaling}"

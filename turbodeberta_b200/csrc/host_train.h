@@ -287,8 +287,9 @@ struct LoraCall {
     }
   }
   Tensor floats(at::IntArrayRef sizes) const { return at::empty(sizes, w.options().dtype(at::kFloat)); }
-  // The product alone, in fp32.
+  // The product alone, in fp32, under autocast too.
   Tensor product(const Tensor& rows, const Tensor& right) const {
+    const c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
     const Tensor left = rows.dim() == 2 ? rows : rows.reshape({l.rows, rows.size(-1)});
     return l.dtype == TDB_DTYPE_F32 ? at::mm(left, right) : at::mm(left, right, at::kFloat);
   }
