@@ -132,3 +132,23 @@ def test_a_model_with_adapters_under_autocast():
             with torch.autocast("cuda", dtype=B):
                 merged = one(input_ids=ids, attention_mask=mask).last_hidden_state[i][v]
             assert (got[i][v].float() - best).norm() <= util.MODEL_BF16_VS_EAGER_FACTOR * (merged.float() - best).norm()
+
+
+# --------------------------------------------------------------------------------------------------------------- infinities
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("rows", [20, 100])
+@pytest.mark.parametrize("rank", [1, 8, 16, 24])
+def test_rows_with_infinities_have_the_formulas_infinities(rank, rows, dtype):
+    """All factors and weights positive: a row with one infinity has infinite results, and no zero that pads a rank makes a NaN of them."""
+    p = inputs(rows, 64, 128, rank, 2, dtype)
+    for k in ("w", "a", "b"):
+        p[k] = p[k].abs() + 0.01
+    p["ids"] = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    p["x"][3, 5] = float("inf")
+    p["dy"][7, 9] = float("inf")
+    leaves = [p[k].clone().requires_grad_() for k in "xab"]
+    y = call(p, *leaves)
+    dx, = torch.autograd.grad(y, leaves[:1], p["dy"])
+    others = torch.arange(rows, device="cuda")
+    assert torch.isposinf(y[3]).all() and torch.isfinite(y[others != 3]).all()
+    assert torch.isposinf(dx[7]).all() and torch.isfinite(dx[others != 7]).all()

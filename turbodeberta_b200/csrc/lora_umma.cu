@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(WARPS * 32) shrink_mma_kernel(const bf16* __re
       float s = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) s += part[w * 16 * MT * 8 * NJ + e];
-      s *= scale;
+      s = j0 + j < rank ? s * scale : 0.f;             // what pads the rank: x's infinities times its zeros would be NaN
       const bf16 high = __float2bfloat16_rn(s);
       const float rest = s - __bfloat162float(high);
       bf16* out = hx + (int64_t)place[row] * 2 * r16 + j0 + j;

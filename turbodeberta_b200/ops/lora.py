@@ -21,7 +21,8 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
     left out when there is one adapter.  A row whose id is not that of an adapter (-1, say) gets the shared projection alone.  The ids are not
     checked on the host: that would wait for the device.
 
-    What an adapter holds, NaN and infinities included, reaches its own rows only, and so do the gradients.
+    What an adapter holds, NaN and infinities included, reaches its own rows only, and so do the gradients.  Where a row of ``x`` or of the result's
+    gradient holds infinities, the gradients of its adapter's factors may be NaN where the formula has infinities.
 
     The bf16 kernels report a device-side wait that gave up through status words that ``check_pending_status()`` (``ops.flash_attention``)
     reads; the call itself does not wait for the device."""
