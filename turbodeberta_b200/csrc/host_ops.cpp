@@ -1392,4 +1392,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dropout", &dropout);
   m.def("norm", &norm);
   m.def("lora_linear", &lora_linear);
+  m.def("lora_form", [](int64_t rows, int columns) {         // of the product on the tensor cores: columns of a tile, SMs that share it
+    int tile = 0, ctas = 0;
+    check_rc(tdb_lora_umma_form(rows, columns, &tile, &ctas));
+    return std::make_pair(tile, ctas);
+  });
 }

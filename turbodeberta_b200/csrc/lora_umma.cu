@@ -797,6 +797,15 @@ int tdb_lora_umma_applies(const Lora* l) {
   return 1;
 }
 
+int tdb_lora_umma_form(int64_t rows, int columns, int* tile_columns, int* ctas) {
+  int sms = 0;
+  if (const int rc = device_sms(&sms)) return rc;
+  const Shape s = shape_of(rows, columns, sms);
+  *tile_columns = s.columns;
+  *ctas = s.ctas;
+  return TDB_OK;
+}
+
 int64_t tdb_lora_inner(const Lora* l) { return 2 * r16_of(*l); }
 
 int tdb_lora_umma_shrink(const Lora* l, int back, const void* f, void* hx, void* stream) {

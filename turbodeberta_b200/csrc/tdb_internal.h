@@ -219,6 +219,8 @@ TDB_HOST_API int tdb_lora_gather_sum(const tdb::Lora* l, const tdb::LoraGradient
 // turned, [n, cols, rank]) in `product`.  hx, u, h: bf16 [rows, tdb_lora_inner()].  status: int32[4], word 0 tells of a wait that gave up.  They lie in the order of the rows, with a
 // plan too.
 TDB_HOST_API int tdb_lora_umma_applies(const tdb::Lora* l);
+// Which tiles `product` takes for an output of that size: their columns, and how many SMs share one.
+TDB_HOST_API int tdb_lora_umma_form(int64_t rows, int columns, int* tile_columns, int* ctas);
 TDB_HOST_API int64_t tdb_lora_inner(const tdb::Lora* l);
 TDB_HOST_API int tdb_lora_umma_shrink(const tdb::Lora* l, int back, const void* f, void* hx, void* stream);
 TDB_HOST_API int tdb_lora_umma_product(const tdb::Lora* l, int back, const void* f, const void* hx, void* y, int32_t* status, void* stream);
