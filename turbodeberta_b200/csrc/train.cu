@@ -239,13 +239,15 @@ __device__ __forceinline__ void cut(Eight& x, int have) {
 // One group of threads to a row, the row in registers; mean first, then the deviations from it (the sum of squares alone would lose
 // the variance of rows far from zero).
 // A block has at most 8 rows of a warp, or one row of up to 512 threads.  With dropout the compiler is told how many blocks an SM is to
-// hold: four where warps have the rows (9216 x 1024 in bf16, 18.3 to 17.5 us), else one (2000 x 4096 in fp32, 25.0 to 24.5).  The norm
-// alone is left without (0): 16384 x 1024 takes 18.4 us so, 19.0 with four and 20.0 with one.
+// hold: four where warps have rows of bf16 (9216 x 1024 17.5 us, 18.3 without), one where a block has the row (2000 x 4096 in fp32 24.5, 25.0
+// without).  Warps with rows of fp32 are left without (0): 64 registers do not hold a row's two units in fp32, and 16384 x 1024 takes 49.4 us so bound and
+// 43.7 without, 9216 x 1024 30.9 and 28.2, 9216 x 1020 59.5 and 55.9, 9216 x 768 18.6 both.  So is the norm alone: 16384 x 1024 takes 18.4 us so, 19.0
+// with four and 20.0 with one.
 constexpr int forward_threads(int kind, int mode) { return kind == A_WARP && mode == JOIN_DROP ? 256 : 512; }
-constexpr int forward_blocks(int kind, int mode) { return mode != JOIN_DROP ? 0 : kind == A_WARP ? 4 : 1; }
+template <typename T> constexpr int forward_blocks(int kind, int mode) { return mode != JOIN_DROP ? 0 : kind != A_WARP ? 1 : sizeof(T) == 2 ? 4 : 0; }
 
 template <typename T, bool VEC, int MODE, int U, int KIND>
-__global__ void __launch_bounds__(forward_threads(KIND, MODE), forward_blocks(KIND, MODE)) norm_forward_kernel(const NormParams p) {
+__global__ void __launch_bounds__(forward_threads(KIND, MODE), forward_blocks<T>(KIND, MODE)) norm_forward_kernel(const NormParams p) {
   extern __shared__ __align__(16) float shared[];
   Group g{p.group, (int)threadIdx.x % p.group, (int)threadIdx.x / p.group, shared, 0};
   const int groups = blockDim.x / p.group;
