@@ -376,10 +376,15 @@ using namespace tdb;
 extern "C" {
 
 // Words of the plan that puts the rows in their adapters' order, 0 where there is none: with one adapter for all, and for few rows, where the launch
-// costs more than it saves (a training step of 700 rows in long requests of three adapters, fp32: 124 us without, 128 with).  Products on the
-// tensor cores go by the rows as they come; their gradients (`train`) want the plan from more rows on.
-int64_t tdb_lora_plan_words(const Lora* l, int train) {
-  return l->ids && l->n > 1 && l->rows >= (train ? 768 : 256) && l->rows < (int64_t)1 << 30 ? l->n + 2 + 2 * l->rows : 0;
+// costs more than it saves.  us of a pass 1024 -> 1024, rank 16, with the plan and without it, for 3 adapters in requests of 60 rows, 32 adapters in
+// requests of 60, and every row with another of 32:
+//   fp32, training             300 rows 102 and 96, 106 and 107, 115 and 179;  700 rows 146 and 148, 160 and 162, 160 and 323;  1000 rows 162 and 159, 171 and 178, 171 and 394
+//   fp32, without gradients    300 rows 47 and 43, 49 and 43, 51 and 66;  700 rows 72 and 68, 76 and 68, 76 and 123;  1000 rows 78 and 72, 80 and 72, 81 and 145
+//   tensor cores, training     300 rows 33 and 27, 44 and 48, 88 and 92;  768 rows 37 and 31, 47 and 59, 90 and 109;  2500 rows 55 and 53, 72 and 128, 145 and 232
+// It costs some 5 us where requests are long and adapters few, and saves up to half where they are not; which of the two a call is only the device knows.
+// Products on the tensor cores go by the rows as they come; their gradients want the plan, from more rows on.
+int64_t tdb_lora_plan_words(const Lora* l, int tensor_cores) {
+  return l->ids && l->n > 1 && l->rows >= (tensor_cores ? 768 : 256) && l->rows < (int64_t)1 << 30 ? l->n + 2 + 2 * l->rows : 0;
 }
 int tdb_lora_plan(const Lora* l, int32_t* plan, void* stream) {
   const int warps = sort_warps(l->n), smem = (warps + 1) * (l->n + 1) * 4;

@@ -206,7 +206,7 @@ TDB_HOST_API int tdb_norm_backward(const tdb::Norm* n, int dtype, void* stream);
 // Adapters beside a shared product, any type and size.  back: from dy through b and a instead of from x through a and b.  h: fp32 [rows, rank].
 // base: the product alone, fp32 [rows, columns of y].  h lies in the order of l->plan, where there is one.
 // The rows sorted by adapter: [n + 2] first positions, [rows] rows, [rows] ids.
-TDB_HOST_API int64_t tdb_lora_plan_words(const tdb::Lora* l, int train);
+TDB_HOST_API int64_t tdb_lora_plan_words(const tdb::Lora* l, int tensor_cores);
 TDB_HOST_API int tdb_lora_plan(const tdb::Lora* l, int32_t* plan, void* stream);
 TDB_HOST_API int tdb_lora_shrink(const tdb::Lora* l, int back, float* h, void* stream);
 TDB_HOST_API int tdb_lora_expand(const tdb::Lora* l, int back, const float* base, const float* h, void* y, void* stream);

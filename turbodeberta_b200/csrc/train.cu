@@ -313,11 +313,12 @@ __global__ void __launch_bounds__(forward_threads(KIND, MODE), forward_blocks<T>
 }
 
 // Backward.  With g = dy w and h = (z - mean) inv:  dz = (g - mean(g) - h mean(g h)) inv, dw = sum over rows of dy h, db of dy.
-// A group of threads keeps the same columns for all its rows, so the weights and both column sums stay in registers, and the 2 R sums of
-// the R rows that it takes at once share one exchange.  A block's sums go to `partial` and are added up by the kernel behind this one, in a
-// fixed order: atomics would make two runs differ.
-// VEC: what a thread will read is on its way several rounds ahead, by asynchronous copies into shared memory that no other thread touches:
-// an SM has some 150 KB in flight while it computes, without barriers or registers for it.
+// A group of threads keeps the same columns for all its rows, so the weights and both column sums stay in registers up to 8192 columns (beyond, with four
+// units to a thread, 372 to 1096 bytes of each thread spill), and the 2 R sums of the R rows that it takes at once share one exchange.  A block's sums
+// go to `partial` and are added up by the kernel behind this one, in a fixed order: atomics would make two runs differ.
+// VEC: what a thread will read is asked for some rounds ahead, by asynchronous copies into shared memory that no other thread touches, without barriers
+// or registers for it.  As the ring holds: three rounds up to 4096 columns, where an SM has some 150 KB in flight while it computes; up to 8192 three in
+// bf16, two in fp32 and one with a residual in fp32; beyond, two in bf16 and one with a residual, and in fp32 none: a round waits for its own copies.
 constexpr int RING_BYTES = 192 * 1024;
 template <typename T, int MODE, int U, int R>
 __host__ __device__ constexpr int round_bytes() { return R * U * (MODE == ALONE ? 2 : 3) * (int)sizeof(Unit<T>); }     // of one thread
