@@ -61,6 +61,11 @@ _MASK_CACHE: dict = {}
 _MASK_LOCK = threading.Lock()
 
 
+def _version(tensor: torch.Tensor):
+    """Of an ordinary tensor; one made in inference mode counts none."""
+    return None if tensor.is_inference() else tensor._version
+
+
 def _mask_cache_put(tensor: torch.Tensor, info) -> None:
     """Remember the analysis of a live mask tensor.  Entries of tensors that have been freed are dropped first; only
     if more than 64 live masks are tracked does the oldest entry go (so a mask that is passed again and again, e.g.
@@ -71,7 +76,7 @@ def _mask_cache_put(tensor: torch.Tensor, info) -> None:
             del _MASK_CACHE[k]
         while len(_MASK_CACHE) >= 64:
             del _MASK_CACHE[next(iter(_MASK_CACHE))]
-        _MASK_CACHE[id(tensor)] = (weakref.ref(tensor), tensor._version, info)
+        _MASK_CACHE[id(tensor)] = (weakref.ref(tensor), _version(tensor), info)
 
 
 def analyse_mask(attention_mask: torch.Tensor | None, batch: int, length: int, refresh: bool = False) -> MaskInfo:
@@ -93,7 +98,7 @@ def analyse_mask(attention_mask: torch.Tensor | None, batch: int, length: int, r
     flags = None
     if hit is not None:
         ref, version, cached = hit
-        if ref() is attention_mask and version == attention_mask._version:     # same live tensor object, unmodified
+        if ref() is attention_mask and version == _version(attention_mask):    # same live tensor object, unmodified
             if not refresh and cached.key_mask is not None:            # the native analysis leaves it out
                 return cached
             flags = (cached.all_ones, cached.right_padded)
@@ -123,7 +128,8 @@ def analyse_mask(attention_mask: torch.Tensor | None, batch: int, length: int, r
         prefix = torch.arange(length, device=key_mask.device)[None, :] < seqlens[:, None]
         flags = torch.stack([key_mask.all(), (prefix == key_mask).all()]).tolist()      # the one sync
     info = MaskInfo(bool(flags[0]), bool(flags[1]), seqlens, key_mask)
-    _mask_cache_put(attention_mask, info)
+    if not attention_mask.is_inference():                           # such a mask may change unseen before the next call
+        _mask_cache_put(attention_mask, info)
     return info
 
 
@@ -133,7 +139,7 @@ def _analyse_2d(attention_mask: torch.Tensor, batch: int, length: int) -> MaskIn
     if attention_mask.shape != (batch, length) or batch == 0 or length == 0:
         return None
     hit = _MASK_CACHE.get(id(attention_mask))
-    if hit is not None and hit[0]() is attention_mask and hit[1] == attention_mask._version and hit[2].all_ones:
+    if hit is not None and hit[0]() is attention_mask and hit[1] == _version(attention_mask) and hit[2].all_ones:
         return hit[2]
     rows = host.mask_rows(attention_mask)
     if rows is None:
@@ -352,7 +358,7 @@ class FlashDebertaV2Encoder(DebertaV2Encoder):
         out = super().get_attention_mask(attention_mask)
         info = getattr(self, "_mask_info", None)
         if info is not None and isinstance(out, torch.Tensor) and out is not attention_mask:
-            _mask_cache_put(out, info)
+            _mask_cache_put(out, info)                              # of this pass alone, so nobody changes it
         return out
 
     @staticmethod
