@@ -1,10 +1,11 @@
-"""The HF model's modules around its matrix products, for passes that record gradients.
+"""The HF model's modules around its matrix products, for training.
 
 ``patch_model(model, train_kernels=True)`` gives the stock modules these classes (parameters and names stay): LayerNorms and dropouts run the
 kernels of ``ops.layer_norm`` and ``ops.dropout``, and the ends of both halves of a layer (``DebertaV2SelfOutput``, ``DebertaV2Output``: dropout,
-residual, LayerNorm) run as one.  Passes of modules in eval mode that record no gradients, other types than float32 and bfloat16, autocast, forward-mode
-derivatives, ``torch.func``'s transforms and the CPU run as before.  In training mode the kernels run without gradients too: a checkpoint's first pass may be one without, and the pass that is made
-again for its gradients has to drop the same elements.
+residual, LayerNorm) run as one.  Passes of modules in eval mode that record no gradients, other types than float32 and bfloat16, autocast,
+forward-mode derivatives, ``torch.func``'s transforms and the CPU run as before.  In training mode the kernels run without gradients too: a
+checkpoint's first pass may be one without, and the pass that is made again for its gradients has to drop the same elements.  A second derivative
+(``create_graph=True``) is refused.
 
 The attention has no backward pass (neither has the reference's), so a training loop reaches what lies behind the last attention whose
 inputs are frozen: task heads, and the last layer's projections, norms and adapters.
