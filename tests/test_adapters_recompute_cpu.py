@@ -184,3 +184,21 @@ def test_kept_functions_leave_what_is_in_use_as_it_was():
     with pytest.raises(ZeroDivisionError):
         A.keep_adapters(lambda: 1 / 0)()
     assert A._ACTIVE.ids is None
+
+
+@pytest.mark.parametrize("way", list(_ways()))
+def test_gradients_may_be_asked_for_more_than_once(way):
+    model = _model()
+    x = _x()
+    params = [x] + [p for p in model[0].parameters() if p.requires_grad]
+    with A.use_adapters([2, -1, 0, 2]):
+        want = torch.autograd.grad(model[0](x).square().sum(), params)
+        loss = _ways()[way](model[0], x).square().sum()
+    if way == "reentrant":                           # such a checkpoint knows backward() alone
+        for turn in (1, 2):
+            loss.backward(retain_graph=True)
+            assert all(torch.allclose(p.grad, turn * w) for p, w in zip(params, want))
+    else:
+        for _ in range(3):
+            assert all(torch.equal(g, w) for g, w in zip(torch.autograd.grad(loss, params, retain_graph=True), want))
+    assert A._ACTIVE.ids is None and A._ACTIVE.before is None

@@ -33,20 +33,27 @@ class _Active(threading.local):
     ids = None                  # of the batch's sequences
     rows = None                 # of the packed stream's tokens
     task = -1                   # the backward pass within which both were chosen; -1: none
+    before = None               # what was in use outside of the present block
 
 
 _ACTIVE = _Active()
 _backward_pass = torch._C._current_graph_task_id             # that this thread is running; -1: none
 
 
-@contextlib.contextmanager
-def _active(ids, rows):
-    before = (_ACTIVE.ids, _ACTIVE.rows, _ACTIVE.task)
-    _ACTIVE.ids, _ACTIVE.rows, _ACTIVE.task = ids, rows, _backward_pass()
-    try:
-        yield
-    finally:
-        _ACTIVE.ids, _ACTIVE.rows, _ACTIVE.task = before
+class _active:
+    """A block in which ``ids`` and ``rows`` are in use; may be entered again, by several threads at once too (a checkpoint's pass is made again as often as
+    its gradients are asked for)."""
+    __slots__ = ("ids", "rows")
+
+    def __init__(self, ids, rows):
+        self.ids, self.rows = ids, rows
+
+    def __enter__(self):
+        _ACTIVE.before = (_ACTIVE.ids, _ACTIVE.rows, _ACTIVE.task, _ACTIVE.before)
+        _ACTIVE.ids, _ACTIVE.rows, _ACTIVE.task = self.ids, self.rows, _backward_pass()
+
+    def __exit__(self, *error):
+        _ACTIVE.ids, _ACTIVE.rows, _ACTIVE.task, _ACTIVE.before = _ACTIVE.before
 
 
 class AdapterLinear(nn.Module):
