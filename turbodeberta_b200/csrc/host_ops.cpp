@@ -265,7 +265,8 @@ py::object Status::report(c10::cuda::CUDAStream stream) {
 }
 
 // Words of every launch with a deferred check, all devices, and of the caller's own report: None, or the largest of each word.
-int standing_slot(int dev);                          // host_train.h; -1: none yet
+int32_t* standing_words(int dev);                    // host_train.h; null: none yet
+constexpr int STANDING = -2;                         // a pending launch that reports there
 py::object drain_pending(Report* own) {
   Words all;
   for (int dev = 0; dev < MAX_DEV; ++dev) {
@@ -276,8 +277,8 @@ py::object drain_pending(Report* own) {
       take.swap(p.pending);
     }
     const bool with_own = own && own->device() == dev;
-    const int standing = standing_slot(dev);
-    if (take.empty() && !with_own && standing < 0) continue;
+    volatile int32_t* const standing = standing_words(dev);
+    if (take.empty() && !with_own && !standing) continue;
     c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
     cudaError_t e = cudaSuccess;
     {
@@ -290,9 +291,14 @@ py::object drain_pending(Report* own) {
       }
       if (with_own && e == cudaSuccess && !(last && own->mark().on(last->stream()) && last->on(own->mark().stream()))) e = own->mark().wait();
     }
-    for (const auto& t : take) all.merge(collect(dev, t.slot, t.keep));
+    for (const auto& t : take)
+      if (t.slot != STANDING) all.merge(collect(dev, t.slot, t.keep));
     if (with_own) all.merge(own->take());
-    if (standing >= 0) all.merge(collect(dev, standing, true));       // replays of graphs report there without being listed
+    for (int i = 0; standing && i < SLOT_WORDS; ++i)                  // replays of graphs report there without being listed
+      if (const int word = standing[i]) {
+        all.w[i] = std::max(all.w[i], word);
+        standing[i] = 0;
+      }
     cuda_ok(e, "synchronisation");
   }
   return all.to_python();

@@ -205,50 +205,36 @@ Tensor norm(const Tensor& x, const OptTensor& res, const Tensor& w, const Tensor
 
 // ----------------------------------------------------------------------------------------------------- projections with adapters
 // Where the product kernels of a device report, calls and recorded graphs alike: words that no call owns, since nothing but a wait that gave up is
-// ever written there.  Each stream that used them since the last check is listed once.
-std::atomic<int> g_standing[MAX_DEV];                // slot + 1
-int standing_slot(int dev) { return g_standing[dev].load() - 1; }
+// ever written there.  They are the host's and zero before the first launch, also where that is being captured.
+std::atomic<int32_t*> g_standing[MAX_DEV];
+int32_t* standing_words(int dev) { return g_standing[dev].load(); }
+int32_t* make_standing_words(int dev) {
+  TORCH_CHECK(dev >= 0 && dev < MAX_DEV, "turbodeberta_b200: up to ", MAX_DEV, " devices are supported");
+  if (int32_t* w = standing_words(dev)) return w;
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  if (int32_t* w = standing_words(dev)) return w;
+  int32_t* w = nullptr;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;         // nothing that a capture of this thread would have to record
+  cuda_ok(cudaThreadExchangeStreamCaptureMode(&mode), "capture mode");
+  const cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&w), SLOT_WORDS * sizeof(int32_t), cudaHostAllocMapped | cudaHostAllocPortable);
+  cuda_ok(cudaThreadExchangeStreamCaptureMode(&mode), "capture mode");
+  cuda_ok(e, "cudaHostAlloc(status words)");
+  std::fill_n(w, SLOT_WORDS, 0);
+  g_standing[dev] = w;
+  return w;
+}
 
-class StandingReport {
- public:
-  StandingReport(int dev, c10::cuda::CUDAStream stream) : dev_(dev), stream_(stream) {
-    captured_ = at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None;
-    slot_ = standing_slot(dev);
-    if (slot_ < 0 && !captured_) {
-      static std::mutex mu;
-      std::lock_guard<std::mutex> lock(mu);
-      if (g_standing[dev] == 0) g_standing[dev] = acquire(dev) + 1;
-      slot_ = standing_slot(dev);
-    }
-    if (slot_ >= 0) {
-      words = g_pools[dev].host + slot_ * SLOT_WORDS;
-    } else {                                         // the first call of a process is being captured, or every slot is taken
-      own_ = at::zeros({SLOT_WORDS}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)dev));
-      words = own_.data_ptr<int32_t>();
-    }
-  }
-  // Behind the launch.
-  void list() {
-    if (own_.defined()) {
-      py::gil_scoped_acquire gil;
-      py::module_::import("turbodeberta_b200.status").attr("PENDING").attr("append")(own_);
-      return;
-    }
-    if (captured_) return;                           // a check looks at the words in any case
-    StatusPool& p = g_pools[dev_];
-    std::lock_guard<std::mutex> lock(p.mu);
-    for (auto& t : p.pending)
-      if (t.slot == slot_ && t.mark.stream() == stream_.stream()) { t.mark.renew(); return; }
-    p.pending.push_back({slot_, Mark(stream_), true});
-  }
-  int32_t* words = nullptr;
-
- private:
-  int dev_, slot_;
-  c10::cuda::CUDAStream stream_;
-  Tensor own_;
-  bool captured_;
-};
+// Behind a launch that reports there.  Each stream that used them since the last check is listed once; a captured launch need not be, since a check looks
+// at the words in any case.
+void list_standing(int dev, c10::cuda::CUDAStream stream) {
+  if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) return;
+  StatusPool& p = g_pools[dev];
+  std::lock_guard<std::mutex> lock(p.mu);
+  for (auto& t : p.pending)
+    if (t.slot == STANDING && t.mark.stream() == stream.stream()) { t.mark.renew(); return; }
+  p.pending.push_back({STANDING, Mark(stream), true});
+}
 
 struct LoraCall {
   Rows x, dy;
@@ -315,9 +301,9 @@ Tensor lora_product(const LoraCall& c, bool back, const Tensor& f, const Tensor&
       check_rc(tdb_lora_skinny(&c.l, h.data_ptr(), y.data_ptr(), stream.stream()));
       return y;
     }
-    StandingReport report(c.w.get_device(), stream);
-    check_rc(tdb_lora_umma_product(&c.l, back, f.data_ptr(), h.data_ptr(), y.data_ptr(), report.words, stream.stream()));
-    report.list();
+    const int dev = c.w.get_device();
+    check_rc(tdb_lora_umma_product(&c.l, back, f.data_ptr(), h.data_ptr(), y.data_ptr(), make_standing_words(dev), stream.stream()));
+    list_standing(dev, stream);
     return y;
   }
   const Tensor base = back ? c.product(c.dy.t, c.w) : c.product(c.x.t, c.w.t());
