@@ -111,3 +111,23 @@ def test_an_adapter_that_is_not_finite_in_tiles_that_two_share(rows, cols, featu
             others = torch.arange(cols, device="cuda") != 5
             assert torch.equal(got["dx"][hurt][:, others], clean["dx"][hurt][:, others]) and not torch.isfinite(got["dx"][hurt][:, 5]).any()
             assert not torch.isfinite(got["y"][hurt]).any()
+
+
+@pytest.mark.parametrize("dtype,cols,features", [(B, 584, 4088), (B, 4088, 200), (F, 264, 130), (B, 65, 66)])
+def test_ids_of_sequences_are_ids_of_their_rows(dtype, cols, features):
+    """Gradients too, with as many rows as are sorted by adapter; 64-bit ids, and ids that lie apart in memory."""
+    p = problem(2600, cols, features, 12, 5, dtype, 1, seed=3)
+    per = torch.tensor([3, -1, 0, 4, 4, 1 << 20, 2, 0], device="cuda", dtype=torch.int32)
+    p["ids"] = per.repeat_interleave(325)
+    want = run(p)
+    apart = torch.stack([per.long(), torch.zeros(8, dtype=torch.int64, device="cuda")], 1)[:, 0]
+    for ids in (per, per.long(), apart, torch.where(per < 0, per.long() - (1 << 40), per.long() + (per > 4) * (1 << 40))):
+        q = dict(p, x=p["x"].view(8, 325, cols), dy=p["dy"].view(8, 325, features), ids=ids)
+        got = run(q)
+        assert all(torch.equal(got[k].reshape(want[k].shape), want[k]) for k in want)
+    p["a"], p["b"], p["s"] = p["a"][:1], p["b"][:1], p["s"][:1]
+    p["ids"] = torch.zeros(2600, dtype=torch.int32, device="cuda")
+    want = run(p)
+    p["ids"] = None                                  # one adapter for all
+    got = run(p)
+    assert all(torch.equal(got[k], want[k]) for k in want)
